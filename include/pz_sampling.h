@@ -351,6 +351,107 @@ pz_status pz_decode_step_count(const pz_decode_step *step, int32_t *steps);
 pz_status pz_decode_step_destroy(pz_decode_step *step);
 
 /* ------------------------------------------------------------------------ */
+/* Rows of logits outside the sampler.  No counterparts in the reference,
+ * whose loop only draws (src/transformer/generate.c:143-170).
+ *
+ * These calls need no context and hold no scratch: they run on the caller's
+ * CURRENT device, which owns the pointers and the stream, allocate nothing,
+ * may be captured into a graph, and calls on different streams may overlap
+ * as long as their outputs are apart.  Rows are given like pz_sample_batch's
+ * (row r at + r*ld elements, any ld >= V, any address that is a multiple of
+ * the element's size).  An empty batch (0 rows) is PZ_OK. */
+
+/* What is applied to each row of logits, in this order.  Device pointers;
+ * each group may be NULL (off).
+ *   penalties: the repetition, frequency and presence penalties of
+ *       cfg[r] over the row's CSR history, exactly step A8 of the pipeline
+ *       contract (the other fields of cfg are not read).  Histories may have
+ *       any length.
+ *   biases: a CSR list of (id, value) per row, added after the penalties.
+ *       Ids outside [0, V) are ignored; of an id listed twice the last entry
+ *       counts.
+ *   mask: bit v % 32 of word v / 32 of a mask row is 1 where id v is
+ *       allowed; the others become -inf whatever they were.  Bits past V are
+ *       ignored.  Logits row r takes mask row mask_index[r], or r where
+ *       mask_index is NULL; an index outside [0, mask_rows) means that the
+ *       row has no mask. */
+typedef struct pz_logits_rules {
+  const pz_sampler_config *cfg;  /* [B]; needed with hist                   */
+  const int32_t *hist;
+  const int32_t *hist_off;       /* [B + 1]                                 */
+  const int32_t *bias_ids;
+  const float *bias_vals;
+  const int32_t *bias_off;       /* [B + 1]                                 */
+  const uint32_t *mask;          /* mask_rows rows, mask_ld words apart     */
+  int64_t mask_ld;               /* >= ceil(V / 32)                         */
+  int32_t mask_rows;             /* >= B where mask_index is NULL           */
+  int32_t reserved;
+  const int32_t *mask_index;     /* [B] or NULL                             */
+} pz_logits_rules;
+
+/* out = logits with the rules applied.  out is the logits buffer itself
+ * (same type and ld: only what changes is touched) or memory apart from it;
+ * out_dtype is the logits' type or PZ_DTYPE_F32 (which keeps the penalised
+ * values of bf16 logits unrounded).  Every step is rounded to fp32, bf16
+ * outputs once more at the end.  n_allowed ([B], may be NULL) receives the
+ * number of ids the row's mask allows (V without a mask): 0 tells a row that
+ * is all -inf, which the samplers treat as they treat any such row.
+ * pz_sample_batch on an f32 `out` without a history draws what it would draw
+ * from the logits with the history. */
+pz_status pz_process_logits(const void *logits, pz_dtype dtype, int B, int V, int64_t ld,
+                            const pz_logits_rules *rules, void *out, pz_dtype out_dtype,
+                            int64_t ld_out, int32_t *n_allowed, void *stream);
+
+/* Distillation: a student's rows of logits against a teacher's short lists
+ * (for instance the cand_ids / cand_logprobs / n_cand of pz_sample_batch).
+ * With q the student's softmax at the temperature T,
+ *   PZ_DISTILL_LIST: values are logits (or log-probabilities; only their
+ *       differences count): p = softmax(values / T) over the list, rho = 0.
+ *   PZ_DISTILL_REST: values are log-probabilities over the whole vocabulary,
+ *       of the distribution at T: p = exp(values); what they leave,
+ *       rho = max(0, 1 - sum p) (0 where the list names every id), is held
+ *       against r, the student's mass off the list, as one class.
+ *   loss[i] = weight[i] T^2 ( sum_j p_j (log p_j - log q_j)
+ *                             + rho (log rho - log r) )
+ * Entries with an id outside [0, V) are ignored; an id listed twice counts
+ * with the sum of its probabilities.  A row whose weight is 0, whose list
+ * has no entries left or, in LIST mode, only values of -inf, has loss and
+ * gradient 0, whatever its logits.  A row of logits that are all -inf has
+ * loss +inf and gradient 0; a listed id the student gives -inf has loss +inf
+ * where its p > 0.  NaN in the logits or in the values of a row makes its
+ * loss and gradient NaN. */
+#define PZ_DISTILL_LIST 0
+#define PZ_DISTILL_REST 1
+#define PZ_DISTILL_MAX_VOCAB 1048576
+typedef struct pz_distill_target {
+  const int32_t *ids;      /* [N x K], rows ld_ids apart                     */
+  const float *values;     /* [N x K], rows ld_values apart                  */
+  int64_t ld_ids;
+  int64_t ld_values;
+  int32_t K;               /* 1 .. PZ_TOP_K_MAX                              */
+  int32_t mode;            /* PZ_DISTILL_*                                   */
+  const int32_t *n_list;   /* [N] entries of each list, or NULL: all K       */
+  const float *weight;     /* [N] or NULL: 1                                 */
+  float temperature;       /* 1e-6 .. 1e6                                    */
+  int32_t reserved;
+} pz_distill_target;
+
+/* loss[N], and the statistics the backward call needs (stats [N x 4], 16-byte
+ * aligned; NULL for evaluation). */
+pz_status pz_distill_forward(const void *logits, pz_dtype dtype, int N, int V, int64_t ld,
+                             const pz_distill_target *target, float *loss, float *stats, void *stream);
+/* grad[i][v] = grad_loss[i] * d loss[i] / d logits[i][v], in the logits' type
+ * (grad_loss NULL: 1), from the forward call's stats on the same logits and
+ * target.  grad is the logits' buffer itself (same ld) or apart from it. */
+pz_status pz_distill_backward(const void *logits, pz_dtype dtype, int N, int V, int64_t ld,
+                              const pz_distill_target *target, const float *stats, const float *grad_loss,
+                              void *grad, int64_t ld_grad, void *stream);
+/* Both in one pass over the logits (grad_loss 1): loss[N] and grad. */
+pz_status pz_distill_loss_grad(const void *logits, pz_dtype dtype, int N, int V, int64_t ld,
+                               const pz_distill_target *target, float *loss, void *grad, int64_t ld_grad,
+                               void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* Multi-GPU.                                                                */
 
 /* Row sharding: the contiguous row range [*begin, *begin + *count) that rank

@@ -17,6 +17,7 @@
 
 #include "../../include/pz_sampling.h"
 #include "pz_kernels.cuh"
+#include "pz_status.cuh"
 
 using pz::FullArgs;
 using pz::MergeArgs;
@@ -132,6 +133,30 @@ bool load_nccl() {
 }
 
 }  // namespace
+
+namespace pz {
+
+pz_status report(pz_status s, const char *msg) {
+  g_last_error = s;
+  std::snprintf(g_detail, sizeof g_detail, "%s", msg);
+  return s;
+}
+
+pz_status report_cuda(cudaError_t e) { return fail_cuda(e); }
+
+int current_sms() {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = -1, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  sms = known[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    known[dev].store(sms, std::memory_order_relaxed);
+  }
+  return sms;
+}
+
+}  // namespace pz
 
 struct pz_sampler_ctx {
   int device = 0;

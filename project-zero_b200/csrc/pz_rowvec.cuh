@@ -1,0 +1,117 @@
+// pz_rowvec.cuh — a row of logits as 16-byte vectors, whatever its address.
+//
+// Rows start anywhere (ld may be odd), so vectors are counted from the last
+// 16-byte boundary at or before the row: `shift` elements before column 0.
+// Vector k covers the columns [k*N - shift, k*N - shift + N); the first and
+// the last may reach outside the row, and those columns are read and
+// written one element at a time.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace pz {
+
+struct bf16_t {  // a bf16 element as it lies in memory
+  uint16_t bits;
+};
+
+template <typename T>
+struct RowElem;
+
+template <>
+struct RowElem<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ float get(const float *p) { return *p; }
+  static __device__ __forceinline__ void put(float *p, float v) { *p = v; }
+  static __device__ __forceinline__ void unpack(const uint4 &u, float *x) {
+    x[0] = __uint_as_float(u.x);
+    x[1] = __uint_as_float(u.y);
+    x[2] = __uint_as_float(u.z);
+    x[3] = __uint_as_float(u.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float *x) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+  static constexpr uint32_t kNegInf2 = 0xFF800000u;  // what a 32-bit word of -inf holds
+};
+
+template <>
+struct RowElem<bf16_t> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ float get(const bf16_t *p) {
+    return __uint_as_float(static_cast<uint32_t>(p->bits) << 16);
+  }
+  // one rounding to nearest even, the output's type being bf16
+  static __device__ __forceinline__ void put(bf16_t *p, float v) {
+    p->bits = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  }
+  static __device__ __forceinline__ void unpack(const uint4 &u, float *x) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      x[2 * j] = __uint_as_float(w[j] << 16);
+      x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+    }
+  }
+  static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+  static __device__ __forceinline__ uint4 pack(const float *x) {
+    return make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+  }
+  static constexpr uint32_t kNegInf2 = 0xFF80FF80u;
+};
+
+// Elements between the last 16-byte boundary at or before p and p.
+template <typename T>
+__device__ __forceinline__ int row_shift(const T *p) {
+  return static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
+}
+
+// Streaming 16-byte load (read once: not kept in L1) and store.
+__device__ __forceinline__ uint4 load16(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void store16(void *p, const uint4 &v) {
+  __stcs(reinterpret_cast<uint4 *>(p), v);
+}
+
+// Vector k of the row: packed, columns outside [0, V) as -inf.
+template <typename T>
+__device__ __forceinline__ uint4 load_row_vec(const T *row, int shift, int V, int k) {
+  constexpr int N = RowElem<T>::N;
+  const int c = k * N - shift;
+  if (c >= 0 && c + N <= V) return load16(row + c);
+  float x[N];
+#pragma unroll
+  for (int j = 0; j < N; j++)
+    x[j] = (c + j >= 0 && c + j < V) ? RowElem<T>::get(row + c + j) : __int_as_float(0xFF800000);
+  return RowElem<T>::pack(x);
+}
+
+// Columns [c, c + N) of the output row, those inside [0, V).  `aligned`:
+// whether a whole vector's address is a multiple of 16 bytes.  N is the
+// input vector's length; the output element may be wider (two stores).
+template <int N, typename T>
+__device__ __forceinline__ void store_row_vec(T *row, int V, int c, const float *x, bool aligned) {
+  constexpr int M = RowElem<T>::N;
+  static_assert(N % M == 0, "an output vector is a whole number of 16-byte stores");
+  if (aligned && c >= 0 && c + N <= V) {
+#pragma unroll
+    for (int i = 0; i < N / M; i++) store16(row + c + i * M, RowElem<T>::pack(x + i * M));
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < N; j++)
+    if (c + j >= 0 && c + j < V) RowElem<T>::put(row + c + j, x[j]);
+}
+
+}  // namespace pz

@@ -1,0 +1,32 @@
+// pz_status.cuh — how the C entries outside pz_capi.cu report a failure
+// (pz_last_error / pz_last_error_detail), and what they share on the host.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/pz_sampling.h"
+
+namespace pz {
+
+// Records the status (and the reason) for this thread and returns it.
+pz_status report(pz_status s, const char *msg);
+pz_status report_cuda(cudaError_t e);
+
+// SMs of the current device, looked up once per device (148 where the
+// lookup fails).
+int current_sms();
+
+// Bytes of B rows of V elements, `ld` elements apart.
+inline uint64_t rows_bytes(int B, int V, int64_t ld, size_t es) {
+  return (static_cast<uint64_t>(B - 1) * static_cast<uint64_t>(ld) + static_cast<uint64_t>(V)) * es;
+}
+// Whether two spans of memory share a byte.
+inline bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + nb && y < x + na;
+}
+inline bool misaligned(const void *p, size_t es) { return reinterpret_cast<uintptr_t>(p) % es != 0; }
+inline size_t elem_bytes(pz_dtype t) { return t == PZ_DTYPE_BF16 ? 2 : 4; }
+
+}  // namespace pz

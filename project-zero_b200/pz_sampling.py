@@ -80,6 +80,23 @@ class Shard(ctypes.Structure):
 SHARD_ROWS, SHARD_VOCAB = 0, 1
 
 
+class LogitsRules(ctypes.Structure):
+    """pz_logits_rules: what pz_process_logits applies to each row."""
+    _fields_ = [("cfg", _vp), ("hist", _vp), ("hist_off", _vp), ("bias_ids", _vp), ("bias_vals", _vp),
+                ("bias_off", _vp), ("mask", _vp), ("mask_ld", ctypes.c_int64), ("mask_rows", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("mask_index", _vp)]
+
+
+class DistillTarget(ctypes.Structure):
+    """pz_distill_target: the teacher's lists."""
+    _fields_ = [("ids", _vp), ("values", _vp), ("ld_ids", ctypes.c_int64), ("ld_values", ctypes.c_int64),
+                ("K", ctypes.c_int32), ("mode", ctypes.c_int32), ("n_list", _vp), ("weight", _vp),
+                ("temperature", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+DISTILL_LIST, DISTILL_REST = 0, 1
+
+
 class SamplerConfigC(ctypes.Structure):
     """pz_sampler_config as a ctypes structure (32 bytes)."""
     _fields_ = [("temperature", ctypes.c_float), ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float),
@@ -193,6 +210,19 @@ _sig("pz_decode_step_create", ctypes.c_int,
 _sig("pz_decode_step_launch", ctypes.c_int, [_vp, _vp])
 _sig("pz_decode_step_count", ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int32)])
 _sig("pz_decode_step_destroy", ctypes.c_int, [_vp])
+
+
+_sig("pz_process_logits", ctypes.c_int,
+     [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.POINTER(LogitsRules), _vp, ctypes.c_int,
+      ctypes.c_int64, _vp, _vp])
+_sig("pz_distill_forward", ctypes.c_int,
+     [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.POINTER(DistillTarget), _vp, _vp, _vp])
+_sig("pz_distill_backward", ctypes.c_int,
+     [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.POINTER(DistillTarget), _vp, _vp, _vp,
+      ctypes.c_int64, _vp])
+_sig("pz_distill_loss_grad", ctypes.c_int,
+     [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.POINTER(DistillTarget), _vp, _vp,
+      ctypes.c_int64, _vp])
 
 
 class PZError(RuntimeError):
@@ -598,3 +628,212 @@ def configs_to_device(cfg_np, device="cuda"):
     import torch
     raw = np.ascontiguousarray(cfg_np, dtype=CONFIG_DTYPE).view(np.uint8)
     return torch.from_numpy(raw.copy()).to(device)
+
+
+# --------------------------------------------------------------------------
+# Rows of logits outside the sampler: constraints, distillation.
+# --------------------------------------------------------------------------
+def _call(fn, name, t, stream, *args):
+    """Calls a context-free entry on t's device, on `stream` or that device's
+    current stream."""
+    import torch
+    dev = t.device.index
+    if dev == torch.cuda.current_device():
+        st = fn(*args, torch.cuda.current_stream().cuda_stream if stream is None else _stream_handle(stream))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch.cuda.current_stream().cuda_stream if stream is None else _stream_handle(stream))
+    if st != PZ_OK:
+        raise PZError(st, name)
+
+
+def _rows(t, name, like=None):
+    """Checks a [rows, columns] CUDA tensor whose columns are contiguous."""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name} has to be [rows, columns] with contiguous columns")
+    if not t.is_cuda:
+        raise ValueError(f"{name} has to be a CUDA tensor")
+    if like is not None and (t.shape != like.shape or t.device != like.device):
+        raise ValueError(f"{name} needs the shape and device of the logits")
+    return t
+
+
+def _ld(t):
+    """Elements between rows (a single row's stride may be anything)."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+
+
+def _vector(t, name, n, dtype, like):
+    """Checks an optional contiguous vector of at least n elements; its
+    device pointer."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() < n or not t.is_contiguous() or t.device != like.device:
+        raise ValueError(f"{name} has to be contiguous {dtype} of at least {n} elements on the logits' device")
+    return t.data_ptr()
+
+
+def process_logits(logits, out=None, *, cfg=None, hist=None, hist_off=None, bias_ids=None, bias_vals=None,
+                   bias_off=None, mask=None, mask_index=None, n_allowed=None, stream=None):
+    """pz_process_logits: penalties (cfg, hist, hist_off as for
+    Sampler.sample), biases (CSR bias_ids int32, bias_vals float32, bias_off
+    int32) and grammar masks (mask: [rows, >= ceil(V/32)] int32 words, bit set
+    = allowed; mask_index: [B] int32 mask row per logits row, -1 = none)
+    applied to logits [B, V].  out=None works in place; out may be float32
+    where the logits are bfloat16.  n_allowed: [B] int32, the ids each row's
+    mask leaves.  Returns out."""
+    import torch
+    _rows(logits, "logits")
+    B, V = logits.shape
+    if out is None:
+        out = logits
+    else:
+        _rows(out, "out", logits)
+    i32 = torch.int32
+    if cfg is not None and (cfg.numel() * cfg.element_size() < 32 * B or not cfg.is_contiguous()
+                            or cfg.device != logits.device):
+        raise ValueError("cfg has to hold one pz_sampler_config (32 bytes) per row on the logits' device")
+    # (an empty tensor has no address: lists without an entry are no lists)
+    if hist is not None and hist.numel() == 0:
+        hist = hist_off = None
+    if bias_ids is not None and bias_ids.numel() == 0:
+        bias_ids = bias_vals = bias_off = None
+    rules = LogitsRules(_ptr(cfg), _vector(hist, "hist", 0, i32, logits),
+                        _vector(hist_off, "hist_off", B + 1, i32, logits),
+                        _vector(bias_ids, "bias_ids", 0, i32, logits),
+                        _vector(bias_vals, "bias_vals", 0, torch.float32, logits),
+                        _vector(bias_off, "bias_off", B + 1, i32, logits))
+    if mask is not None:
+        _rows(mask, "mask")
+        if mask.dtype not in (i32, torch.uint32) or mask.device != logits.device:
+            raise ValueError("mask has to be int32 or uint32 words on the logits' device")
+        rules.mask, rules.mask_ld, rules.mask_rows = mask.data_ptr(), _ld(mask), mask.shape[0]
+        if mask.shape[1] * 32 < V:
+            raise ValueError(f"mask rows of {mask.shape[1]} words do not cover {V} ids")
+        rules.mask_index = _vector(mask_index, "mask_index", B, i32, logits)
+    elif mask_index is not None:
+        raise ValueError("mask_index without mask")
+    if V == 0:
+        raise ValueError("logits without columns")
+    if B == 0:
+        return out
+    _call(_lib.pz_process_logits, "pz_process_logits", logits, stream, logits.data_ptr(), Sampler._dtype_code(logits),
+          B, V, _ld(logits), ctypes.byref(rules), out.data_ptr(), Sampler._dtype_code(out), _ld(out),
+          _vector(n_allowed, "n_allowed", B, i32, logits))
+    return out
+
+
+def _target(logits, ids, values, weight, temperature, mode, n_list):
+    import torch
+    _rows(logits, "logits")
+    _rows(ids, "ids")
+    _rows(values, "values")
+    N = logits.shape[0]
+    if ids.dtype != torch.int32 or values.dtype != torch.float32:
+        raise TypeError("ids have to be int32 and values float32")
+    if ids.shape != values.shape or ids.shape[0] != N or ids.device != logits.device or values.device != ids.device:
+        raise ValueError("ids and values have to be [rows of the logits, K] on the logits' device")
+    if logits.shape[1] == 0:
+        raise ValueError("logits without columns")
+    return DistillTarget(ids.data_ptr(), values.data_ptr(), _ld(ids), _ld(values), ids.shape[1], mode,
+                         _vector(n_list, "n_list", N, torch.int32, logits),
+                         _vector(weight, "weight", N, torch.float32, logits), temperature, 0)
+
+
+def distill_forward(logits, ids, values, loss, stats=None, *, weight=None, temperature=1.0, mode=DISTILL_LIST,
+                    n_list=None, stream=None):
+    """pz_distill_forward: loss [N] float32 of the student's logits [N, V]
+    against the teacher's lists ids [N, K] int32 / values [N, K] float32
+    (mode DISTILL_LIST or DISTILL_REST), and, for distill_backward, stats
+    [N, 4] float32.  Returns loss."""
+    import torch
+    target = _target(logits, ids, values, weight, temperature, mode, n_list)
+    N, V = logits.shape
+    if N == 0:
+        return loss
+    _call(_lib.pz_distill_forward, "pz_distill_forward", logits, stream, logits.data_ptr(),
+          Sampler._dtype_code(logits), N, V, _ld(logits), ctypes.byref(target),
+          _vector(loss, "loss", N, torch.float32, logits), _vector(stats, "stats", 4 * N, torch.float32, logits))
+    return loss
+
+
+def distill_backward(logits, ids, values, stats, grad, grad_loss=None, *, weight=None, temperature=1.0,
+                     mode=DISTILL_LIST, n_list=None, stream=None):
+    """pz_distill_backward: grad [N, V] (the logits' type; may be the logits
+    themselves) of sum(grad_loss * loss) from distill_forward's stats on the
+    same arguments.  Returns grad."""
+    import torch
+    target = _target(logits, ids, values, weight, temperature, mode, n_list)
+    N, V = logits.shape
+    _rows(grad, "grad", logits)
+    if grad.dtype != logits.dtype:
+        raise TypeError("grad needs the logits' type")
+    if N == 0:
+        return grad
+    _call(_lib.pz_distill_backward, "pz_distill_backward", logits, stream, logits.data_ptr(),
+          Sampler._dtype_code(logits), N, V, _ld(logits), ctypes.byref(target),
+          _vector(stats, "stats", 4 * N, torch.float32, logits),
+          _vector(grad_loss, "grad_loss", N, torch.float32, logits), grad.data_ptr(), _ld(grad))
+    return grad
+
+
+def distill_loss_grad(logits, ids, values, loss, grad, *, weight=None, temperature=1.0, mode=DISTILL_LIST,
+                      n_list=None, stream=None):
+    """pz_distill_loss_grad: loss [N] and the gradient of its sum, in one
+    pass over the logits (grad may be the logits themselves).  Returns
+    (loss, grad)."""
+    import torch
+    target = _target(logits, ids, values, weight, temperature, mode, n_list)
+    N, V = logits.shape
+    _rows(grad, "grad", logits)
+    if grad.dtype != logits.dtype:
+        raise TypeError("grad needs the logits' type")
+    if N == 0:
+        return loss, grad
+    _call(_lib.pz_distill_loss_grad, "pz_distill_loss_grad", logits, stream, logits.data_ptr(),
+          Sampler._dtype_code(logits), N, V, _ld(logits), ctypes.byref(target),
+          _vector(loss, "loss", N, torch.float32, logits), grad.data_ptr(), _ld(grad))
+    return loss, grad
+
+
+_distill_fn = None
+
+
+def _distill_function():
+    """The autograd function behind distill_loss (made at the first call, so
+    that importing this module does not import torch)."""
+    global _distill_fn
+    if _distill_fn is None:
+        import torch
+
+        class Distill(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, logits, ids, values, weight, temperature, mode, n_list):
+                N = logits.shape[0]
+                loss = torch.empty(N, dtype=torch.float32, device=logits.device)
+                stats = torch.empty(N, 4, dtype=torch.float32, device=logits.device)
+                distill_forward(logits, ids, values, loss, stats, weight=weight, temperature=temperature, mode=mode,
+                                n_list=n_list)
+                ctx.save_for_backward(logits, ids, values, weight, n_list, stats)
+                ctx.how = (temperature, mode)
+                return loss
+
+            @staticmethod
+            @torch.autograd.function.once_differentiable
+            def backward(ctx, grad_loss):
+                logits, ids, values, weight, n_list, stats = ctx.saved_tensors
+                temperature, mode = ctx.how
+                grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+                distill_backward(logits, ids, values, stats, grad, grad_loss.contiguous(), weight=weight,
+                                 temperature=temperature, mode=mode, n_list=n_list)
+                return grad, None, None, None, None, None, None
+
+        _distill_fn = Distill
+    return _distill_fn
+
+
+def distill_loss(logits, ids, values, *, weight=None, temperature=1.0, mode=DISTILL_LIST, n_list=None):
+    """The row losses [N] of distill_forward, differentiable in the logits
+    (not in the teacher's values or the weights).  Runs on the current
+    stream; the gradient is one more pass over the logits."""
+    return _distill_function().apply(logits, ids, values, weight, temperature, mode, n_list)
