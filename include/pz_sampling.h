@@ -451,6 +451,33 @@ pz_status pz_distill_loss_grad(const void *logits, pz_dtype dtype, int N, int V,
                                const pz_distill_target *target, float *loss, void *grad, int64_t ld_grad,
                                void *stream);
 
+/* The LM head in 8-bit integers, a scale per token and per channel: half the
+ * bytes of pz_lm_head_logits' bf16 classifier.
+ *
+ * pz_quantize_rows_i8: per row, top = max |x|, scale = top / 127,
+ * q = rint(x * (127 / top)), each step rounded to fp32.  Rows with top below
+ * 2^-100 become zeros with scale 0; a row that holds an inf or a NaN becomes
+ * zeros with scale NaN (its products are NaN).  Classifier rows are
+ * quantised with it once, hidden rows at every call.
+ * pz_matmul_i8: out[m][n] = float(sum_k a[m][k] w[n][k]) * (a_scale[m] *
+ * w_scale[n]), the sum in 32-bit integers (K < PZ_MATMUL_I8_MAX_K).
+ * pz_lm_head_logits_i8: both, hidden [B x dim] (f32 or bf16) into logits
+ * (f32 or bf16), with the caller's buffers for the quantised tokens
+ * (hidden_q [B x dim], hidden_scale [B]; overwritten, so two calls in flight
+ * need two of them).
+ * 8-bit matrices start on a 16-byte boundary and so does each of their rows
+ * (ld_* multiples of 16); what lies between K and ld is not read. */
+#define PZ_MATMUL_I8_MAX_K 131072
+pz_status pz_quantize_rows_i8(const void *x, pz_dtype dtype, int rows, int cols, int64_t ld, int8_t *q,
+                              int64_t ld_q, float *scale, void *stream);
+pz_status pz_matmul_i8(const int8_t *a, int64_t ld_a, const float *a_scale, int M, const int8_t *w, int64_t ld_w,
+                       const float *w_scale, int N, int K, void *out, pz_dtype out_dtype, int64_t ld_out,
+                       void *stream);
+pz_status pz_lm_head_logits_i8(const void *hidden, pz_dtype hidden_dtype, int B, int dim, int64_t ld_hidden,
+                               const int8_t *w_q, int64_t ld_w, const float *w_scale, int V, void *logits,
+                               pz_dtype logits_dtype, int64_t ld, int8_t *hidden_q, int64_t ld_q,
+                               float *hidden_scale, void *stream);
+
 /* ------------------------------------------------------------------------ */
 /* Multi-GPU.                                                                */
 

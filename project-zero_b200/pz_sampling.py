@@ -225,6 +225,16 @@ _sig("pz_distill_loss_grad", ctypes.c_int,
       ctypes.c_int64, _vp])
 
 
+_sig("pz_quantize_rows_i8", ctypes.c_int,
+     [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp])
+_sig("pz_matmul_i8", ctypes.c_int,
+     [_vp, ctypes.c_int64, _vp, ctypes.c_int, _vp, ctypes.c_int64, _vp, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int,
+      ctypes.c_int64, _vp])
+_sig("pz_lm_head_logits_i8", ctypes.c_int,
+     [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, _vp, ctypes.c_int64, _vp, ctypes.c_int, _vp,
+      ctypes.c_int, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp])
+
+
 class PZError(RuntimeError):
     def __init__(self, status, what=""):
         self.status = status
@@ -837,3 +847,73 @@ def distill_loss(logits, ids, values, *, weight=None, temperature=1.0, mode=DIST
     (not in the teacher's values or the weights).  Runs on the current
     stream; the gradient is one more pass over the logits."""
     return _distill_function().apply(logits, ids, values, weight, temperature, mode, n_list)
+
+
+# --------------------------------------------------------------------------
+# The LM head in 8-bit integers.
+# --------------------------------------------------------------------------
+def _i8(t, name, like, shape):
+    """Checks an int8 [rows, columns] tensor whose rows start on 16 bytes;
+    its row stride."""
+    import torch
+    _rows(t, name)
+    if t.dtype != torch.int8 or tuple(t.shape) != shape or t.device != like.device:
+        raise ValueError(f"{name} has to be int8 {list(shape)} on the same device")
+    # (a single row's stride is free; the library wants a multiple of 16)
+    return (t.shape[1] + 15) // 16 * 16 if t.shape[0] <= 1 else t.stride(0)
+
+
+def quantize_rows_i8(x, q, scale, stream=None):
+    """pz_quantize_rows_i8: x [rows, cols] float32 or bfloat16 into q [rows,
+    cols] int8 (rows a multiple of 16 bytes apart, e.g. torch.empty(rows,
+    (cols + 15) // 16 * 16, dtype=torch.int8)[:, :cols]) and scale [rows]
+    float32.  Returns (q, scale)."""
+    import torch
+    _rows(x, "x")
+    rows, cols = x.shape
+    ld_q = _i8(q, "q", x, (rows, cols))
+    out = _vector(scale, "scale", rows, torch.float32, x)
+    if rows == 0:
+        return q, scale
+    _call(_lib.pz_quantize_rows_i8, "pz_quantize_rows_i8", x, stream, x.data_ptr(), Sampler._dtype_code(x), rows,
+          cols, _ld(x), q.data_ptr(), ld_q, out)
+    return q, scale
+
+
+def matmul_i8(a, a_scale, w, w_scale, out, stream=None):
+    """pz_matmul_i8: out [M, N] (float32 or bfloat16) = (a [M, K] @ w [N, K]^T)
+    * a_scale [M] * w_scale [N], the sums in 32-bit integers.  Returns out."""
+    import torch
+    _rows(out, "out")
+    M, N = out.shape
+    K = a.shape[1]
+    ld_a, ld_w = _i8(a, "a", out, (M, K)), _i8(w, "w", out, (N, K))
+    sa, sw = (_vector(t, n, k, torch.float32, out) for t, n, k in ((a_scale, "a_scale", M), (w_scale, "w_scale", N)))
+    if M == 0:
+        return out
+    _call(_lib.pz_matmul_i8, "pz_matmul_i8", out, stream, a.data_ptr(), ld_a, sa, M, w.data_ptr(), ld_w, sw, N, K,
+          out.data_ptr(), Sampler._dtype_code(out), _ld(out))
+    return out
+
+
+def lm_head_i8(hidden, w_q, w_scale, logits, hidden_q, hidden_scale, stream=None):
+    """pz_lm_head_logits_i8: logits [B, V] (float32 or bfloat16) = hidden
+    [B, dim] (float32 or bfloat16), quantised per row into hidden_q [B, dim]
+    int8 / hidden_scale [B], times the classifier w_q [V, dim] int8 with
+    w_scale [V] (quantize_rows_i8).  Returns logits."""
+    import torch
+    _rows(hidden, "hidden")
+    _rows(logits, "logits")
+    B, dim = hidden.shape
+    V = w_q.shape[0]
+    if tuple(logits.shape) != (B, V) or logits.device != hidden.device:
+        raise ValueError("logits have to be [B, V] on the hidden rows' device")
+    ld_w, ld_q = _i8(w_q, "w_q", hidden, (V, dim)), _i8(hidden_q, "hidden_q", hidden, (B, dim))
+    sw, sq = (_vector(t, n, k, torch.float32, hidden)
+              for t, n, k in ((w_scale, "w_scale", V), (hidden_scale, "hidden_scale", B)))
+    if B == 0:
+        return logits
+    _call(_lib.pz_lm_head_logits_i8, "pz_lm_head_logits_i8", hidden, stream, hidden.data_ptr(),
+          Sampler._dtype_code(hidden), B, dim, _ld(hidden), w_q.data_ptr(), ld_w, sw, V, logits.data_ptr(),
+          Sampler._dtype_code(logits), _ld(logits), hidden_q.data_ptr(), ld_q, sq)
+    return logits

@@ -76,3 +76,29 @@ def test_distill_refuses_outputs_and_limits():
 
 def test_structures_match_the_header():
     assert ctypes.sizeof(pz.LogitsRules) == 80 and ctypes.sizeof(pz.DistillTarget) == 64
+
+
+def head(hidden=P, dtype=0, B=2, dim=64, ld_h=64, w=P, ld_w=64, ws=P, V=100, out=P, out_dtype=0, ld=100, q=P, ld_q=64,
+         s=P):
+    return L.pz_lm_head_logits_i8(hidden, dtype, B, dim, ld_h, w, ld_w, ws, V, out, out_dtype, ld, q, ld_q, s, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(hidden=None), dict(w=None), dict(ws=None), dict(out=None), dict(q=None), dict(s=None), dict(B=-1),
+    dict(dim=0), dict(V=0), dict(ld_h=63), dict(ld_w=48), dict(ld_w=72), dict(ld_q=72), dict(ld_q=48), dict(ld=99),
+    dict(dtype=2), dict(out_dtype=2), dict(w=P + 8), dict(q=P + 8), dict(hidden=P + 2), dict(out=P + 2),
+    dict(ws=P + 2), dict(s=P + 2),
+], ids=str)
+def test_head_refuses(kw):
+    assert head(**kw) == BAD
+    assert b"_i8" in L.pz_last_error_detail()
+
+
+def test_head_limits_and_empty():
+    big = dict(dim=1 << 17, ld_h=1 << 17, ld_w=1 << 17, ld_q=1 << 17)
+    assert head(**big) == UNSUPPORTED
+    assert head(B=0) == OK
+    assert L.pz_matmul_i8(P, 64, P, 0, P, 64, P, 10, 64, P, 0, 10, None) == OK
+    assert L.pz_matmul_i8(P, 64, None, 2, P, 64, P, 10, 64, P, 0, 10, None) == BAD
+    assert L.pz_quantize_rows_i8(P, 0, 0, 64, 64, P, 64, P, None) == OK
+    assert L.pz_quantize_rows_i8(P, 0, 2, 64, 64, P, 60, P, None) == BAD
