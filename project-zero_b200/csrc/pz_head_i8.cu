@@ -13,8 +13,13 @@
 // Product: out[m][n] = float(sum_k a[m][k] w[n][k]) * (a_scale[m] * w_scale[n]),
 // the sum in 32-bit integers (exact for K < 2^17), then three fp32 roundings,
 // and one to bf16 where that is the output.
+#include <cuda.h>
+
+#include <atomic>
+
 #include "pz_rowvec.cuh"
 #include "pz_status.cuh"
+#include "pz_tcgen05.cuh"
 
 namespace pz {
 namespace {
@@ -37,6 +42,7 @@ template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const QuantArgs A) {
   constexpr int N = RowElem<T>::N;
   constexpr int NT = kQuantThreads;
+  pdl_launch_dependents();  // the product may start fetching its weights
   __shared__ float s_top[NT / 32];
   __shared__ int s_bad[NT / 32];
   const int64_t row = blockIdx.x;
@@ -127,47 +133,293 @@ struct MatmulArgs {
   void *out;
 };
 
-constexpr int kMatRows = 8;
+// ---------------------------------------------------------------------------
+// The product on the tensor cores.  out^T = W a^T: a tile is 128 channels
+// (the instruction's M, so a decode batch of few tokens still fills it) by
+// up to 256 tokens (its N, a multiple of 16).
+//
+// Few tokens: bound by HBM, every weight read once: a persistent CTA per SM
+// keeps about 200 KB of weights and tokens in flight.  Many tokens: bound by
+// the tensor cores and, behind them, by L2 (a tile of 128 x 256 reads 384
+// bytes per 32768 products).
+//
+// Warp 0 issues TMA loads (128 channels x 128 bytes of K and the tokens'
+// part, 128-byte swizzle) into a ring of stages; one thread of warp 1 issues
+// four tcgen05.mma (K = 32 each) per stage; the sums lie in tensor memory,
+// two tiles of them, so that warps 2 to 5 read, scale and store one tile
+// while the next is summed.  A lane of the epilogue holds one channel: a
+// warp stores 32 neighbouring logits of a token at a time.
+//
+// Rows and K past the matrices' ends arrive as zeros.  Every wait is bounded:
+// one that runs out (4 s; nothing in this kernel can cause it) ends the CTA
+// after its loads have landed and its products are done, with NaN in the
+// outputs it did not reach.
+// ---------------------------------------------------------------------------
+constexpr int kTcThreads = 192;
+constexpr int kTcChannels = 128;
+constexpr int kTcTokens = 256;
+constexpr int kTcK = 128;             // bytes of K per stage
+constexpr int kTcMaxStages = 12;
+constexpr int kTcRing = 200 * 1024;   // shared memory of the ring
 
-// One warp takes a channel at a time and 8 tokens, 4 products per instruction.
+struct TcArgs {
+  const float *a_scale, *w_scale;
+  void *out;
+  int64_t ld_out;
+  int M, N;
+  int nt;          // tokens per tile, a multiple of 16
+  int tok_tiles;
+  int tiles;       // channel tiles x tok_tiles
+  int k_blocks;    // stages' worth of K
+  int k_steps;     // K in steps of 32
+  int stages;
+  int cols;        // tensor memory columns, a power of two >= 2 nt
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256) matmul_i8_kernel(const MatmulArgs A) {
-  const int lane = threadIdx.x & 31;
-  const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (n >= A.N) return;
-  const int m0 = blockIdx.y * kMatRows;
-  const int8_t *w = A.w + static_cast<int64_t>(n) * A.ld_w;
-  int acc[kMatRows];
-#pragma unroll
-  for (int r = 0; r < kMatRows; r++) acc[r] = 0;
-  const int whole = A.K / 4;
-  for (int k = lane; k < whole; k += 32) {
-    const int x = reinterpret_cast<const int *>(w)[k];
-#pragma unroll
-    for (int r = 0; r < kMatRows; r++)
-      if (m0 + r < A.M)
-        acc[r] = __dp4a(x, reinterpret_cast<const int *>(A.a + static_cast<int64_t>(m0 + r) * A.ld_a)[k], acc[r]);
+__global__ void __launch_bounds__(kTcThreads, 1)
+    matmul_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const TcArgs A) {
+  extern __shared__ unsigned char s_raw[];
+  __shared__ __align__(8) uint64_t s_full[kTcMaxStages], s_empty[kTcMaxStages], s_sum[2], s_free[2], s_drain;
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_stop;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t ring = (smem_addr(s_raw) + 1023u) & ~1023u;
+  const uint32_t w_bytes = kTcChannels * kTcK, a_bytes = static_cast<uint32_t>(A.nt) * kTcK;
+  const uint32_t stage_bytes = w_bytes + a_bytes;
+  const uint32_t full = smem_addr(s_full), empty = smem_addr(s_empty), sum = smem_addr(s_sum), free_ = smem_addr(s_free);
+
+  if (tid == 0) {
+    tma_prefetch_map(&map_w);
+    tma_prefetch_map(&map_a);
+    for (int i = 0; i < A.stages; i++) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(sum + 8 * i, 1);
+      mbar_init(free_ + 8 * i, 4);
+    }
+    mbar_init(smem_addr(&s_drain), 1);
+    mbar_init_fence();
+    s_stop = 0;
   }
-  for (int k = whole * 4 + lane; k < A.K; k += 32)
+  if (warp == 2) tmem_alloc(smem_addr(&s_tmem), static_cast<uint32_t>(A.cols));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // The weights of the first stages do not depend on what runs before
+      // this kernel (the tokens' quantisation): they are on their way first.
+      const int mine = (A.tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+      const int64_t total = static_cast<int64_t>(mine) * A.k_blocks;
+      const int early = static_cast<int>(total < A.stages ? total : A.stages);
+      int it = 0, ph = 0;  // stage and its phase
+      auto weights = [&](int stage, int tile, int kb) {
+        mbar_expect(full + 8 * stage, stage_bytes);
+        tma_load(ring + stage * stage_bytes, &map_w, kb * kTcK, tile / A.tok_tiles * kTcChannels, full + 8 * stage);
+      };
+      {
+        int tile = blockIdx.x, kb = 0;
+        for (int i = 0; i < early; i++) {
+          weights(i, tile, kb);
+          if (++kb == A.k_blocks) {
+            kb = 0;
+            tile += gridDim.x;
+          }
+        }
+      }
+      pdl_wait();
+      int64_t n = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < A.tiles; tile += gridDim.x) {
+        for (int kb = 0; kb < A.k_blocks; kb++) {
+          if (n >= early) {
+            if (!(ok = mbar_wait(empty + 8 * it, ph ^ 1, &s_stop))) break;
+            weights(it, tile, kb);
+          }
+          tma_load(ring + it * stage_bytes + w_bytes, &map_a, kb * kTcK, tile % A.tok_tiles * A.nt, full + 8 * it);
+          n++;
+          if (++it == A.stages) {
+            it = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      // after a stop: no load may be in flight when the CTA's memory goes
+      if (s_stop) {
+        const int64_t last = n < A.stages ? n : A.stages;
+        for (int64_t i = n - last; i < n; i++) {
+          volatile int ignore = 0;
+          mbar_wait(full + 8 * static_cast<uint32_t>(i % A.stages), static_cast<uint32_t>((i / A.stages) & 1), &ignore);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t inst = i8_instruction(A.nt);
+      int it = 0, ph = 0, t = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < A.tiles; tile += gridDim.x, t++) {
+        const int acc = t & 1;
+        if (!(ok = mbar_wait(free_ + 8 * acc, ((t >> 1) & 1) ^ 1, &s_stop))) break;
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(acc * (A.cols / 2));
+        for (int kb = 0; kb < A.k_blocks; kb++) {
+          if (!(ok = mbar_wait(full + 8 * it, ph, &s_stop))) break;
+          tc_fence_after();
+          const uint64_t dw = smem_desc(ring + it * stage_bytes), da = smem_desc(ring + it * stage_bytes + w_bytes);
+          const int steps = min(kTcK / 32, A.k_steps - kb * (kTcK / 32));
+          for (int k = 0; k < steps; k++) tc_mma_i8(d, dw + 2 * k, da + 2 * k, inst, kb > 0 || k > 0);
+          tc_commit(empty + 8 * it);
+          if (++it == A.stages) {
+            it = 0;
+            ph ^= 1;
+          }
+        }
+        if (ok) tc_commit(sum + 8 * acc);
+      }
+      if (s_stop) {
+        volatile int ignore = 0;
+        tc_commit(smem_addr(&s_drain));
+        mbar_wait(smem_addr(&s_drain), 0, &ignore);
+      }
+    }
+    __syncwarp();
+  } else {
+    pdl_wait();
+    const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
+    const int row = quarter * 32 + lane;
+    int t = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < A.tiles; tile += gridDim.x, t++) {
+      const int acc = t & 1;
+      const int n = tile / A.tok_tiles * kTcChannels + row;
+      const int m0 = tile % A.tok_tiles * A.nt;
+      T *out = static_cast<T *>(A.out) + static_cast<int64_t>(m0) * A.ld_out + n;
+      const int tokens = min(A.nt, A.M - m0);
+      if (ok) ok = mbar_wait(sum + 8 * acc, (t >> 1) & 1, &s_stop);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) {
+        for (int j = 0; j < tokens; j++)
+          if (n < A.N) RowElem<T>::put(out + static_cast<int64_t>(j) * A.ld_out, __int_as_float(0x7FC00000));
+        continue;
+      }
+      tc_fence_after();
+      const float sw = n < A.N ? A.w_scale[n] : 0.0f;
+      const uint32_t at = tmem + static_cast<uint32_t>(acc * (A.cols / 2)) + (static_cast<uint32_t>(quarter * 32) << 16);
+      for (int c = 0; c < tokens; c += 16) {
+        int v[16];
+        __syncwarp();
+        tmem_load16(at + c, v);
+        tmem_load_wait();
 #pragma unroll
-    for (int r = 0; r < kMatRows; r++)
-      if (m0 + r < A.M) acc[r] += w[k] * A.a[static_cast<int64_t>(m0 + r) * A.ld_a + k];
-#pragma unroll
-  for (int r = 0; r < kMatRows; r++) {
-    const int s = __reduce_add_sync(0xFFFFFFFFu, acc[r]);
-    if (lane == 0 && m0 + r < A.M)
-      RowElem<T>::put(static_cast<T *>(A.out) + static_cast<int64_t>(m0 + r) * A.ld_out + n,
-                      __fmul_rn(__int2float_rn(s), __fmul_rn(A.a_scale[m0 + r], A.w_scale[n])));
+        for (int j = 0; j < 16; j++)
+          if (c + j < tokens && n < A.N)
+            RowElem<T>::put(out + static_cast<int64_t>(c + j) * A.ld_out,
+                            __fmul_rn(__int2float_rn(v[j]), __fmul_rn(__ldcg(A.a_scale + m0 + c + j), sw)));
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(free_ + 8 * acc);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_free(tmem, static_cast<uint32_t>(A.cols));
   }
 }
 
-cudaError_t launch_matmul(const MatmulArgs &A, pz_dtype out_dtype, cudaStream_t st) {
-  const dim3 grid((A.N + 7) / 8, (A.M + kMatRows - 1) / kMatRows);
-  if (out_dtype == PZ_DTYPE_F32)
-    matmul_i8_kernel<float><<<grid, 256, 0, st>>>(A);
-  else
-    matmul_i8_kernel<bf16_t><<<grid, 256, 0, st>>>(A);
-  return cudaGetLastError();
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder, looked up once (the library does not link libcuda).
+EncodeTiled encoder() {
+  static std::atomic<void *> known{nullptr};
+  void *f = known.load(std::memory_order_acquire);
+  if (f == nullptr) {
+    cudaDriverEntryPointQueryResult how;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &how) != cudaSuccess ||
+        how != cudaDriverEntryPointSuccess)
+      return nullptr;
+    known.store(f, std::memory_order_release);
+  }
+  return reinterpret_cast<EncodeTiled>(f);
+}
+
+// 8-bit rows of K values as tiles of `box` rows by 128 bytes.
+bool encode_rows(CUtensorMap *map, const int8_t *p, int K, int rows, int64_t ld, int box) {
+  const EncodeTiled f = encoder();
+  if (f == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+  const cuuint32_t size[2] = {kTcK, static_cast<cuuint32_t>(box)}, step[2] = {1, 1};
+  return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(p), dims, strides, size, step,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// after_quantize: launched behind the tokens' quantisation, whose end the
+// kernel waits for itself.
+template <typename T>
+cudaError_t launch_matmul_as(const MatmulArgs &P, bool after_quantize, cudaStream_t st) {
+  TcArgs A{};
+  A.a_scale = P.a_scale;
+  A.w_scale = P.w_scale;
+  A.out = P.out;
+  A.ld_out = P.ld_out;
+  A.M = P.M;
+  A.N = P.N;
+  A.tok_tiles = (P.M + kTcTokens - 1) / kTcTokens;
+  A.nt = ((P.M + A.tok_tiles - 1) / A.tok_tiles + 15) / 16 * 16;
+  const int64_t tiles = static_cast<int64_t>((P.N + kTcChannels - 1) / kTcChannels) * A.tok_tiles;
+  if (tiles > 0x3FFFFFFF) return cudaErrorInvalidConfiguration;
+  A.tiles = static_cast<int>(tiles);
+  A.k_blocks = (P.K + kTcK - 1) / kTcK;
+  A.k_steps = (P.K + 31) / 32;
+  const int stage = (kTcChannels + A.nt) * kTcK;
+  A.stages = kTcRing / stage < kTcMaxStages ? kTcRing / stage : kTcMaxStages;
+  A.cols = 32;
+  while (A.cols < 2 * A.nt) A.cols *= 2;
+  CUtensorMap map_w, map_a;
+  if (!encode_rows(&map_w, P.w, P.K, P.N, P.ld_w, kTcChannels) || !encode_rows(&map_a, P.a, P.K, P.M, P.ld_a, A.nt))
+    return cudaErrorInvalidValue;
+  const size_t smem = static_cast<size_t>(A.stages) * stage + 1024;
+  static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !((ready.load(std::memory_order_acquire) >> dev) & 1u)) {
+    e = cudaFuncSetAttribute(matmul_i8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcRing + 1024);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg{};
+  const int sms = current_sms();
+  cfg.gridDim = dim3(static_cast<unsigned>(A.tiles < sms ? A.tiles : sms));
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = after_quantize ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, matmul_i8_kernel<T>, map_w, map_a, A);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+cudaError_t launch_matmul(const MatmulArgs &A, pz_dtype out_dtype, bool after_quantize, cudaStream_t st) {
+  return out_dtype == PZ_DTYPE_F32 ? launch_matmul_as<float>(A, after_quantize, st)
+                                   : launch_matmul_as<bf16_t>(A, after_quantize, st);
 }
 
 pz_status check_quantize(const void *x, pz_dtype dtype, int rows, int cols, int64_t ld, const int8_t *q, int64_t ld_q,
@@ -215,7 +467,7 @@ pz_status pz_matmul_i8(const int8_t *a, int64_t ld_a, const float *a_scale, int 
   const pz::MatmulArgs A{a, a_scale, w, w_scale, M, N, K, ld_a, ld_w, ld_out, out};
   const pz_status s = pz::check_matmul(A, out_dtype);
   if (s != PZ_OK || M == 0) return s;
-  const cudaError_t e = pz::launch_matmul(A, out_dtype, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = pz::launch_matmul(A, out_dtype, false, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? PZ_OK : pz::report_cuda(e);
 }
 
@@ -230,7 +482,7 @@ pz_status pz_lm_head_logits_i8(const void *hidden, pz_dtype hidden_dtype, int B,
   if (s != PZ_OK || B == 0) return s;
   const pz::QuantArgs Q{hidden, ld_hidden, B, dim, hidden_q, ld_q, hidden_scale};
   cudaError_t e = pz::launch_quantize(Q, hidden_dtype, static_cast<cudaStream_t>(stream));
-  if (e == cudaSuccess) e = pz::launch_matmul(A, logits_dtype, static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) e = pz::launch_matmul(A, logits_dtype, true, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? PZ_OK : pz::report_cuda(e);
 }
 
