@@ -312,16 +312,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_fence_after();
       const float sw = n < A.N ? A.w_scale[n] : 0.0f;
       const uint32_t at = tmem + static_cast<uint32_t>(acc * (A.cols / 2)) + (static_cast<uint32_t>(quarter * 32) << 16);
-      for (int c = 0; c < tokens; c += 16) {
-        int v[16];
+      // 32 tokens at a time; each lane fetches one token's scale, ahead of
+      // the stores that the compiler may not move a load across
+      float sa = lane < tokens ? __ldcg(A.a_scale + m0 + lane) : 0.0f;
+      for (int c = 0; c < tokens; c += 32) {
+        int v[32];
         __syncwarp();
-        tmem_load16(at + c, v);
+        tmem_load32(at + c, v);
+        const float here = sa;
+        if (c + 32 + lane < tokens) sa = __ldcg(A.a_scale + m0 + c + 32 + lane);
         tmem_load_wait();
+        float x[32];
 #pragma unroll
-        for (int j = 0; j < 16; j++)
-          if (c + j < tokens && n < A.N)
-            RowElem<T>::put(out + static_cast<int64_t>(c + j) * A.ld_out,
-                            __fmul_rn(__int2float_rn(v[j]), __fmul_rn(__ldcg(A.a_scale + m0 + c + j), sw)));
+        for (int j = 0; j < 32; j++)
+          x[j] = __fmul_rn(__int2float_rn(v[j]), __fmul_rn(__shfl_sync(0xFFFFFFFFu, here, j), sw));
+        T *o = out + static_cast<int64_t>(c) * A.ld_out;
+        if (c + 32 <= tokens) {
+          if (n < A.N) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) RowElem<T>::put(o + j * A.ld_out, x[j]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j++)
+            if (c + j < tokens && n < A.N) RowElem<T>::put(o + j * A.ld_out, x[j]);
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -387,7 +402,7 @@ cudaError_t launch_matmul_as(const MatmulArgs &P, bool after_quantize, cudaStrea
   A.k_steps = (P.K + 31) / 32;
   const int stage = (kTcChannels + A.nt) * kTcK;
   A.stages = kTcRing / stage < kTcMaxStages ? kTcRing / stage : kTcMaxStages;
-  A.cols = 32;
+  A.cols = 64;  // (the epilogue reads 32 columns at a time)
   while (A.cols < 2 * A.nt) A.cols *= 2;
   CUtensorMap map_w, map_a;
   if (!encode_rows(&map_w, P.w, P.K, P.N, P.ld_w, kTcChannels) || !encode_rows(&map_a, P.a, P.K, P.M, P.ld_a, A.nt))
