@@ -39,10 +39,11 @@
 namespace pz {
 namespace {
 
-constexpr int kRes = 8;                // vectors of a thread that stay in registers
-constexpr int kDistillThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBatch = 4;              // 16-byte vectors that a thread has in flight
 constexpr int kMaxCluster = 8;         // the portable cluster size
-constexpr int kBackThreads = 256;
+constexpr int kCtasPerSm = 4;
 
 struct DistillArgs {
   const void *logits;
@@ -63,6 +64,7 @@ struct DistillArgs {
   int64_t ld_grad;
   int parts;  // CTAs per row (the cluster's size in distill_kernel)
   int span;   // vectors per CTA
+  int bit_words;  // words of a CTA's bits of listed columns, a multiple of 4
 };
 
 // 2^x, fp32 results below 2^-126 flushed to zero (they are lost in any sum
@@ -73,93 +75,19 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// What a CTA knows about its row's list.
-struct ListShared {
-  int32_t id[PZ_TOP_K_MAX];   // -1: ignored
-  float p[PZ_TOP_K_MAX];
-  float own_p[PZ_TOP_K_MAX];  // probability of the entry's id, at the first entry of an id in this CTA's columns; else -1
-  float own_s[PZ_TOP_K_MAX];  // the student's logit there
+// A CTA's view of its row's list, in shared memory; entry j belongs to thread
+// j % kThreads, which alone reads and writes it once the list is set up.
+struct List {
+  int32_t *id;     // [K]; -1: ignored, or a later entry of an id listed twice
+  float *p;        // [K] probabilities
+  uint32_t *bits;  // one bit per column of the CTA's span: listed
   double sum_p;
   float rho;
-  int valid;                  // the row has a target
-  int twice;                  // an id is listed twice in this CTA's columns
+  bool valid;      // the row has a target
 };
 
-// Reads the row's list into L: ids, probabilities, their sum and rho.  Warp 0
-// works out the probabilities; every thread of the block calls this, and a
-// barrier has to follow.
-__device__ __forceinline__ void read_list(const DistillArgs &A, int row, ListShared &L) {
-  const int tid = threadIdx.x, lane = tid & 31;
-  if (tid >= 32) return;
-  const int32_t *ids = A.ids + row * A.ld_ids;
-  const float *values = A.values + row * A.ld_values;
-  const int n = A.n_list ? min(max(A.n_list[row], 0), A.K) : A.K;
-  float top = -INFINITY;
-  int seen = 0, bad = 0;
-  for (int j = lane; j < A.K; j += 32) {
-    int id = j < n ? ids[j] : -1;
-    if (id >= A.V) id = -1;
-    if (id < 0) id = -1;
-    float t = -INFINITY;
-    if (id >= 0) {
-      t = A.rest ? values[j] : __fdiv_rn(values[j], A.T);
-      seen++;
-      bad |= t != t;
-      top = fmaxf(top, t);
-    }
-    L.id[j] = id;
-    L.p[j] = t;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    seen += __shfl_xor_sync(0xFFFFFFFFu, seen, o);
-    bad |= __shfl_xor_sync(0xFFFFFFFFu, bad, o);
-  }
-  // LIST: relative to the largest; REST: as they are
-  const float base = (A.rest || !(top > -INFINITY)) ? 0.0f : top;
-  double sum = 0.0;
-  for (int j = lane; j < A.K; j += 32) {
-    const float p = L.id[j] >= 0 ? expf(__fsub_rn(L.p[j], base)) : 0.0f;
-    L.p[j] = p;
-    sum += p;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  if (!A.rest) {
-    const float inv = static_cast<float>(1.0 / sum);
-    sum = 0.0;
-    for (int j = lane; j < A.K; j += 32) {
-      if (L.id[j] >= 0) L.p[j] = __fmul_rn(L.p[j], inv);
-      sum += L.p[j];
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  }
-  // A list that names every id leaves none for rho (what 1 - sum holds then
-  // is rounding).
-  bool whole = A.rest && seen >= A.V;
-  if (whole) {
-    __syncwarp();
-    for (int v = lane; v < A.V; v += 32) {
-      bool on = false;
-      for (int j = 0; j < A.K; j++) on |= L.id[j] == v;
-      whole &= on;
-    }
-    whole = __all_sync(0xFFFFFFFFu, whole);
-  }
-  if (lane == 0) {
-    L.sum_p = sum;  // of the probabilities as they are held
-    // (an unordered comparison keeps a NaN sum: the row's outputs are NaN then)
-    L.rho = (A.rest && !whole && !(sum >= 1.0)) ? static_cast<float>(1.0 - sum) : 0.0f;
-    // no entries: no target.  LIST with no finite value: none either.
-    L.valid = seen > 0 && (A.rest || top > -INFINITY || bad);
-    L.twice = 0;
-  }
-}
-
-// The first column of this CTA's span and one past its last, for the row
-// whose columns start `shift` elements after a 16-byte boundary.
+// The columns [c0, c1) that a CTA takes of a row whose columns start `shift`
+// elements after a 16-byte boundary: the vectors [k0, k1).
 template <typename T>
 struct Span {
   int k0, k1, c0, c1;
@@ -173,51 +101,145 @@ struct Span {
   }
 };
 
-// The list's entries in the columns [c0, c1): one bit per column in `bits`,
-// the student's logits in own_s.  The bits are zero before; barriers before
-// (read_list) and after.
-template <typename T>
-__device__ __forceinline__ void mark_list(const DistillArgs &A, ListShared &L, uint32_t *bits, const T *row, int c0,
-                                          int c1, int nt) {
-  for (int j = threadIdx.x; j < A.K; j += nt) {
-    const int id = L.id[j];
-    float own = -1.0f;
-    if (id >= 0 && id >= c0 && id < c1) {
-      const int u = id - c0;
-      if (atomicOr(&bits[u >> 5], 1u << (u & 31)) & (1u << (u & 31))) L.twice = 1;
-      L.own_s[j] = RowElem<T>::get(row + id);
-      own = L.p[j];
+// Reads the row's list: ids and probabilities, their sum, rho, and the bits
+// of the ids in [c0, c1).  Two barriers of the block, the second one last.
+__device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, int c0, int c1, unsigned char *smem,
+                                          int bit_words) {
+  __shared__ float s_top[kWarps];
+  __shared__ int s_seen[kWarps], s_bad[kWarps];
+  __shared__ double s_sum[kWarps];
+  __shared__ int s_twice, s_gap;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  List L;
+  L.bits = reinterpret_cast<uint32_t *>(smem);
+  L.id = reinterpret_cast<int32_t *>(L.bits + bit_words);
+  L.p = reinterpret_cast<float *>(L.id + A.K);
+  const int32_t *ids = A.ids + row * A.ld_ids;
+  const float *values = A.values + row * A.ld_values;
+  const int n = A.n_list ? min(max(A.n_list[row], 0), A.K) : A.K;
+  float top = -INFINITY;
+  int seen = 0, bad = 0;
+  for (int j = tid; j < A.K; j += kThreads) {
+    int id = ids[j];
+    const float v = values[j];
+    float t = -INFINITY;
+    if (j >= n || id < 0 || id >= A.V) {
+      id = -1;
+    } else {
+      t = A.rest ? v : __fdiv_rn(v, A.T);
+      seen++;
+      bad |= t != t;
+      top = fmaxf(top, t);
     }
-    L.own_p[j] = own;
+    L.id[j] = id;
+    L.p[j] = t;
   }
-}
-
-// Where an id is listed twice its first entry takes the whole probability,
-// in list order.  Called between two barriers.
-__device__ __forceinline__ void join_doubles(const DistillArgs &A, ListShared &L, int nt) {
-  if (!L.twice) return;
-  for (int j = threadIdx.x; j < A.K; j += nt) {
+  for (int i = tid; i < bit_words / 4; i += kThreads) reinterpret_cast<uint4 *>(L.bits)[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  seen = __reduce_add_sync(0xFFFFFFFFu, seen);
+  bad = __any_sync(0xFFFFFFFFu, bad);
+  if (lane == 0) {
+    s_top[warp] = top;
+    s_seen[warp] = seen;
+    s_bad[warp] = bad;
+  }
+  if (tid == 0) s_twice = s_gap = 0;
+  __syncthreads();
+  seen = 0;
+  for (int i = 0; i < kWarps; i++) {
+    top = fmaxf(top, s_top[i]);
+    seen += s_seen[i];
+    bad |= s_bad[i];
+  }
+  // LIST: relative to the largest; REST: as they are
+  const float base = (A.rest || !(top > -INFINITY)) ? 0.0f : top;
+  double sum = 0.0;
+  for (int j = tid; j < A.K; j += kThreads) {
     const int id = L.id[j];
-    if (id < 0 || L.own_p[j] == -1.0f) continue;  // outside this CTA's columns
-    float sum = 0.0f;
-    bool first = true;
-    for (int i = 0; i < A.K; i++)
-      if (L.id[i] == id) {
-        if (i < j) first = false;
-        sum = __fadd_rn(sum, L.p[i]);
-      }
-    L.own_p[j] = first ? sum : -1.0f;
+    const float p = id >= 0 ? expf(__fsub_rn(L.p[j], base)) : 0.0f;
+    L.p[j] = p;
+    sum += p;
+    if (id >= 0 && id >= c0 && id < c1) {
+      const uint32_t bit = 1u << ((id - c0) & 31);
+      if (atomicOr(&L.bits[(id - c0) >> 5], bit) & bit) s_twice = 1;
+    }
   }
+  // A list that names every id leaves none for rho (what 1 - sum holds then
+  // is rounding).
+  const bool whole = A.rest && seen >= A.V;
+  if (whole) {
+    for (int v = tid; v < A.V; v += kThreads) {
+      bool on = false;
+      for (int j = 0; j < A.K; j++) on |= L.id[j] == v;
+      if (!on) s_gap = 1;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int i = 0; i < kWarps; i++) sum += s_sum[i];
+  if (!A.rest) {
+    const float inv = static_cast<float>(1.0 / sum);
+    for (int j = tid; j < A.K; j += kThreads)
+      if (L.id[j] >= 0) L.p[j] = __fmul_rn(L.p[j], inv);
+    if (sum == sum) sum = 1.0;  // a NaN value makes the row's outputs NaN
+  }
+  L.sum_p = sum;
+  // (an unordered comparison keeps a NaN sum: the row's outputs are NaN then)
+  L.rho = (A.rest && !(whole && !s_gap) && !(sum >= 1.0)) ? static_cast<float>(1.0 - sum) : 0.0f;
+  // no entries: no target.  LIST with no finite value: none either.
+  L.valid = seen > 0 && (A.rest || top > -INFINITY || bad);
+  if (s_twice) {
+    // the first entry of an id takes the probabilities of all, in list order
+    __syncthreads();
+    float joined[PZ_TOP_K_MAX / kThreads];
+#pragma unroll
+    for (int e = 0; e < PZ_TOP_K_MAX / kThreads; e++) {
+      const int j = tid + e * kThreads;
+      joined[e] = -1.0f;
+      if (j < A.K && L.id[j] >= 0) {
+        float all = 0.0f;
+        bool first = true;
+        for (int i = 0; i < A.K; i++)
+          if (L.id[i] == L.id[j]) {
+            first &= i >= j;
+            all = __fadd_rn(all, L.p[i]);
+          }
+        if (first) joined[e] = all;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PZ_TOP_K_MAX / kThreads; e++) {
+      const int j = tid + e * kThreads;
+      if (j < A.K) {
+        if (joined[e] == -1.0f) L.id[j] = -1;
+        L.p[j] = joined[e];
+      }
+    }
+  }
+  return L;
 }
 
 template <typename T>
-__device__ __forceinline__ void zero_span(T *row, const Span<T> &sp, int V, bool aligned, int nt) {
+__device__ __forceinline__ void zero_span(T *row, const Span<T> &sp, int V, bool aligned) {
   constexpr int N = RowElem<T>::N;
   float x[N];
 #pragma unroll
   for (int j = 0; j < N; j++) x[j] = 0.0f;
-  for (int k = sp.k0 + threadIdx.x; k < sp.k1; k += nt)
+  for (int k = sp.k0 + threadIdx.x; k < sp.k1; k += kThreads)
     store_row_vec<N>(row, V, sp.c0 + (k - sp.k0) * N, x, aligned);
+}
+
+// kBatch vectors of the span, from vector k on, kThreads apart.
+template <typename T>
+__device__ __forceinline__ void load_batch(const T *row, int shift, int V, int k, int k1, uint4 *raw) {
+#pragma unroll
+  for (int i = 0; i < kBatch; i++)
+    if (k + i * kThreads < k1) raw[i] = load_row_vec(row, shift, V, k + i * kThreads);
 }
 
 // A maximum and the sum of e relative to it.
@@ -279,20 +301,12 @@ struct RowSums {
   float M, S, M_off, S_off;
 };
 
-template <typename T>
-__device__ __forceinline__ void grad_vec(const uint4 &raw, float m, float c, float f, float *x) {
-  constexpr int N = RowElem<T>::N;
-  RowElem<T>::unpack(raw, x);
-#pragma unroll
-  for (int j = 0; j < N; j++) x[j] = __fmul_rn(exp2_approx(__fmul_rn(__fsub_rn(x[j], m), c)), f);
-}
-
 // What the passes multiply e by.
 struct GradFactors {
   float q_of_e;  // listed ids, e relative to M: P / S
   float f;       // the others, e relative to M_off: w T (P / S 2^((M_off - M) c) - rho / S_off)
 };
-__device__ __forceinline__ GradFactors grad_factors(const ListShared &L, const RowSums &R, float c, float by) {
+__device__ __forceinline__ GradFactors grad_factors(const List &L, const RowSums &R, float c, float by) {
   // a row without any weight (every logit -inf): its gradient is 0
   if (R.S == 0.0f) return GradFactors{0.0f, 0.0f};
   const float P = __fadd_rn(static_cast<float>(L.sum_p), L.rho);
@@ -304,28 +318,117 @@ __device__ __forceinline__ GradFactors grad_factors(const ListShared &L, const R
   return g;
 }
 
-// The listed ids get their own gradient, over what the pass along the row
-// wrote there (a barrier before).
+// One batch of the pass along the row: e times f.
 template <typename T>
-__device__ __forceinline__ void grad_list(const DistillArgs &A, const ListShared &L, T *grad, float M, float by,
-                                          float q_of_e, int nt) {
-  for (int j = threadIdx.x; j < A.K; j += nt) {
-    const float p = L.own_p[j];
-    if (p == -1.0f) continue;
-    const float e = exp2_approx(__fmul_rn(__fsub_rn(L.own_s[j], M), A.c));
-    RowElem<T>::put(grad + L.id[j], q_of_e == 0.0f ? 0.0f : __fmul_rn(by, __fsub_rn(__fmul_rn(e, q_of_e), p)));
+__device__ __forceinline__ void grad_batch(const uint4 *raw, const Span<T> &sp, int k, int V, T *grad, bool aligned,
+                                           float m, float c, float f) {
+  constexpr int N = RowElem<T>::N;
+#pragma unroll
+  for (int i = 0; i < kBatch; i++) {
+    const int at = k + i * kThreads;
+    if (at < sp.k1) {
+      float x[N];
+      RowElem<T>::unpack(raw[i], x);
+#pragma unroll
+      for (int j = 0; j < N; j++) x[j] = __fmul_rn(exp2_approx(__fmul_rn(__fsub_rn(x[j], m), c)), f);
+      store_row_vec<N>(grad, V, sp.c0 + (at - sp.k0) * N, x, aligned);
+    }
   }
 }
 
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads, 2) distill_kernel(const DistillArgs A) {
+// The pass along the row, the next batch in flight while one is worked on;
+// then the listed ids get their own gradient over what the pass wrote there.
+// Their logits are read before it: the gradient may lie over the logits.
+template <typename T>
+__device__ __forceinline__ void write_gradient(const DistillArgs &A, const List &L, const Span<T> &sp, const T *row,
+                                               int shift, T *grad, bool aligned, const RowSums &R, float by) {
+  constexpr int STEP = kBatch * kThreads;
+  const GradFactors g = grad_factors(L, R, A.c, by);
+  constexpr int E = PZ_TOP_K_MAX / kThreads;
+  float own[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int j = static_cast<int>(threadIdx.x) + e * kThreads;
+    own[e] = 0.0f;
+    if (j < A.K) {
+      const int id = L.id[j];
+      if (id >= 0 && id >= sp.c0 && id < sp.c1) own[e] = RowElem<T>::get(row + id);
+    }
+  }
+  int k = sp.k0 + static_cast<int>(threadIdx.x);
+  uint4 a[kBatch], b[kBatch];
+  load_batch(row, shift, A.V, k, sp.k1, a);
+  // every listed logit of the span has been read (their values are used
+  // below, behind this barrier's wait for the loads)
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const float x = exp2_approx(__fmul_rn(__fsub_rn(own[e], R.M), A.c));
+    own[e] = __fmul_rn(x, g.q_of_e);
+  }
+  __syncthreads();
+  for (; k < sp.k1; k += 2 * STEP) {
+    load_batch(row, shift, A.V, k + STEP, sp.k1, b);
+    grad_batch(a, sp, k, A.V, grad, aligned, R.M_off, A.c, g.f);
+    load_batch(row, shift, A.V, k + 2 * STEP, sp.k1, a);
+    grad_batch(b, sp, k + STEP, A.V, grad, aligned, R.M_off, A.c, g.f);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int j = static_cast<int>(threadIdx.x) + e * kThreads;
+    if (j < A.K) {
+      const int id = L.id[j];
+      if (id >= 0 && id >= sp.c0 && id < sp.c1)
+        RowElem<T>::put(grad + id, g.q_of_e == 0.0f ? 0.0f : __fmul_rn(by, __fsub_rn(own[e], L.p[j])));
+    }
+  }
+}
+
+// One batch into a thread's running maximum and sum.  REST: listed ids are
+// left out.
+template <typename T>
+__device__ __forceinline__ void sum_batch(const DistillArgs &A, const List &L, const Span<T> &sp, uint4 *raw, int k,
+                                          MaxSum &a) {
   constexpr int N = RowElem<T>::N;
-  constexpr int NT = kDistillThreads;
-  constexpr int NW = NT / 32;
-  __shared__ ListShared L;
+  float x[N];
+  float top = a.m;
+#pragma unroll
+  for (int i = 0; i < kBatch; i++) {
+    const int at = k + i * kThreads;
+    if (at >= sp.k1) {
+      raw[i] = make_uint4(RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2);
+    } else if (A.rest) {
+      const int u = (at - sp.k0) * N;
+      const uint32_t on = (L.bits[u >> 5] >> (u & 31)) & ((1u << N) - 1u);
+      if (on != 0u) {
+        RowElem<T>::unpack(raw[i], x);
+#pragma unroll
+        for (int j = 0; j < N; j++)
+          if ((on >> j) & 1u) x[j] = -INFINITY;
+        raw[i] = RowElem<T>::pack(x);
+      }
+    }
+    RowElem<T>::unpack(raw[i], x);
+#pragma unroll
+    for (int j = 0; j < N; j++) top = fmaxf(top, x[j]);
+  }
+  const float base = top > -INFINITY ? top : 0.0f;
+  float s = __fmul_rn(a.s, exp2_approx(__fmul_rn(__fsub_rn(a.m, base), A.c)));
+#pragma unroll
+  for (int i = 0; i < kBatch; i++) {
+    RowElem<T>::unpack(raw[i], x);
+#pragma unroll
+    for (int j = 0; j < N; j++) s = __fadd_rn(s, exp2_approx(__fmul_rn(__fsub_rn(x[j], base), A.c)));
+  }
+  a = MaxSum{top, s};
+}
+
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const DistillArgs A) {
+  constexpr int STEP = kBatch * kThreads;
   __shared__ __align__(16) RowPart s_part[kMaxCluster];
-  __shared__ MaxSum s_warp[NW][2];
-  extern __shared__ uint32_t s_bits[];
+  __shared__ MaxSum s_warp[kWarps][2];
+  extern __shared__ __align__(16) unsigned char s_dyn[];
   const int part = static_cast<int>(blockIdx.x) % A.parts;
   const int64_t row = blockIdx.x / A.parts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -336,35 +439,18 @@ __global__ void __launch_bounds__(kDistillThreads, 2) distill_kernel(const Disti
   const bool aligned =
       GRAD && ((reinterpret_cast<uintptr_t>(g_row) - static_cast<uintptr_t>(shift) * sizeof(T)) & 15u) == 0;
   const float w = A.weight ? A.weight[row] : 1.0f;
-  const float by = __fmul_rn(w, A.T);
 
-  if (w == 0.0f) {  // the whole cluster leaves: the row is not read
-    if (GRAD) zero_span(g_row, sp, A.V, aligned, NT);
-    if (part == 0 && tid == 0) {
-      A.loss[row] = 0.0f;
-      if (A.stats) A.stats[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-    return;
+  bool target = w != 0.0f;
+  List L;
+  uint4 ra[kBatch], rb[kBatch];
+  int k = sp.k0 + tid;
+  if (target) {
+    load_batch(x_row, shift, A.V, k, sp.k1, ra);
+    L = read_list(A, row, sp.c0, sp.c1, s_dyn, A.bit_words);
+    target = L.valid;
   }
-  // The span's batches of kRes vectors per thread, the first one last: it
-  // stays in registers for the gradient.
-  const int batches = max(1, (sp.k1 - sp.k0 + kRes * NT - 1) / (kRes * NT));
-  uint4 raw[kRes];
-  auto load = [&](int b) {
-#pragma unroll
-    for (int i = 0; i < kRes; i++) {
-      const int k = sp.k0 + (b * kRes + i) * NT + tid;
-      raw[i] = k < sp.k1 ? load_row_vec(x_row, shift, A.V, k)
-                         : make_uint4(RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2,
-                                      RowElem<T>::kNegInf2);
-    }
-  };
-  load(batches - 1);
-  for (int i = tid; i < (A.span * N + 31) / 32; i += NT) s_bits[i] = 0u;
-  read_list(A, static_cast<int>(row), L);
-  __syncthreads();
-  if (!L.valid) {
-    if (GRAD) zero_span(g_row, sp, A.V, aligned, NT);
+  if (!target) {  // the whole cluster leaves
+    if (GRAD) zero_span(g_row, sp, A.V, aligned);
     if (part == 0 && tid == 0) {
       A.loss[row] = 0.0f;
       if (A.stats) A.stats[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -372,52 +458,22 @@ __global__ void __launch_bounds__(kDistillThreads, 2) distill_kernel(const Disti
     return;
   }
   cluster_arrive();
-  mark_list(A, L, s_bits, x_row, sp.c0, sp.c1, NT);
-  __syncthreads();
-  join_doubles(A, L, NT);
 
   // running maximum and sum of this thread's columns
   MaxSum a{-INFINITY, 0.0f};
-  for (int b = batches - 1; b >= 0; b--) {
-    if (b < batches - 1) load(b);
-    float x[N];
-    if (A.rest) {  // listed ids leave the sum
-#pragma unroll
-      for (int i = 0; i < kRes; i++) {
-        const int u = ((b * kRes + i) * NT + tid) * N;
-        const uint32_t on = u < A.span * N ? (s_bits[u >> 5] >> (u & 31)) & ((1u << N) - 1u) : 0u;
-        if (on != 0u) {
-          RowElem<T>::unpack(raw[i], x);
-#pragma unroll
-          for (int j = 0; j < N; j++)
-            if ((on >> j) & 1u) x[j] = -INFINITY;
-          raw[i] = RowElem<T>::pack(x);
-        }
-      }
-    }
-    float top = a.m;
-#pragma unroll
-    for (int i = 0; i < kRes; i++) {
-      RowElem<T>::unpack(raw[i], x);
-#pragma unroll
-      for (int j = 0; j < N; j++) top = fmaxf(top, x[j]);
-    }
-    const float base = top > -INFINITY ? top : 0.0f;
-    float s = __fmul_rn(a.s, exp2_approx(__fmul_rn(__fsub_rn(a.m, base), A.c)));
-#pragma unroll
-    for (int i = 0; i < kRes; i++) {
-      RowElem<T>::unpack(raw[i], x);
-#pragma unroll
-      for (int j = 0; j < N; j++) s = __fadd_rn(s, exp2_approx(__fmul_rn(__fsub_rn(x[j], base), A.c)));
-    }
-    a = MaxSum{top, s};
+  for (; k < sp.k1; k += 2 * STEP) {
+    load_batch(x_row, shift, A.V, k + STEP, sp.k1, rb);
+    sum_batch(A, L, sp, ra, k, a);
+    load_batch(x_row, shift, A.V, k + 2 * STEP, sp.k1, ra);
+    if (k + STEP < sp.k1) sum_batch(A, L, sp, rb, k + STEP, a);
   }
   // and of its listed ids
   MaxSum listed{-INFINITY, 0.0f};
   if (A.rest) {
-    for (int j = tid; j < A.K; j += NT) {
-      if (L.own_p[j] == -1.0f) continue;
-      const float sv = L.own_s[j];
+    for (int j = tid; j < A.K; j += kThreads) {
+      const int id = L.id[j];
+      if (id < 0 || id < sp.c0 || id >= sp.c1) continue;
+      const float sv = RowElem<T>::get(x_row + id);
       listed = join(listed, MaxSum{sv, sv == -INFINITY ? 0.0f : 1.0f}, A.c);
     }
     listed = join_warp(listed, A.c);
@@ -428,29 +484,50 @@ __global__ void __launch_bounds__(kDistillThreads, 2) distill_kernel(const Disti
     s_warp[warp][1] = listed;
   }
   __syncthreads();
-  cluster_wait();  // every CTA of the row runs: its shared memory may be written
-  if (warp == 0) {
-    RowPart r{s_warp[0][0], s_warp[0][1], 0.0, 0.0, 0.0, 0.0};
-    for (int i = 1; i < NW; i++) {
-      r.row = join(r.row, s_warp[i][0], A.c);
-      r.list = join(r.list, s_warp[i][1], A.c);
-    }
-    const double ref = r.ref();
-    for (int j = lane; j < A.K; j += 32) {
-      const float p = L.own_p[j];
-      if (p == -1.0f || p == 0.0f) continue;
-      r.p += p;
-      r.plogp += static_cast<double>(p) * logf(p);
-      r.ps += static_cast<double>(p) * (L.own_s[j] - ref);
-    }
+  RowPart r{s_warp[0][0], s_warp[0][1], 0.0, 0.0, 0.0, 0.0};
+  for (int i = 1; i < kWarps; i++) {
+    r.row = join(r.row, s_warp[i][0], A.c);
+    r.list = join(r.list, s_warp[i][1], A.c);
+  }
+  const double ref = r.ref();
+  for (int j = tid; j < A.K; j += kThreads) {
+    const int id = L.id[j];
+    const float p = L.p[j];
+    if (id < 0 || id < sp.c0 || id >= sp.c1 || p == 0.0f) continue;
+    r.p += p;
+    r.plogp += static_cast<double>(p) * logf(p);
+    r.ps += static_cast<double>(p) * (RowElem<T>::get(x_row + id) - ref);
+  }
+  if (A.K > 32) {  // entries in several warps
+    __shared__ double s_list[kWarps][3];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       r.p += __shfl_xor_sync(0xFFFFFFFFu, r.p, o);
       r.plogp += __shfl_xor_sync(0xFFFFFFFFu, r.plogp, o);
       r.ps += __shfl_xor_sync(0xFFFFFFFFu, r.ps, o);
     }
-    if (lane < A.parts) put_remote(&s_part[part], r, lane);
+    if (lane == 0) {
+      s_list[warp][0] = r.p;
+      s_list[warp][1] = r.plogp;
+      s_list[warp][2] = r.ps;
+    }
+    __syncthreads();
+    r.p = r.plogp = r.ps = 0.0;
+    for (int i = 0; i < kWarps; i++) {
+      r.p += s_list[i][0];
+      r.plogp += s_list[i][1];
+      r.ps += s_list[i][2];
+    }
+  } else if (warp == 0) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      r.p += __shfl_xor_sync(0xFFFFFFFFu, r.p, o);
+      r.plogp += __shfl_xor_sync(0xFFFFFFFFu, r.plogp, o);
+      r.ps += __shfl_xor_sync(0xFFFFFFFFu, r.ps, o);
+    }
   }
+  cluster_wait();  // every CTA of the row runs: its shared memory may be written
+  if (tid < A.parts) put_remote(&s_part[part], r, tid);
   cluster_arrive();
   cluster_wait();
   RowPart all = s_part[0];
@@ -468,11 +545,13 @@ __global__ void __launch_bounds__(kDistillThreads, 2) distill_kernel(const Disti
   if (!(R.M_off > -INFINITY)) R.M_off = R.M;
   if (part == 0 && tid == 0) {
     const double T_ = A.T, log_s = log(static_cast<double>(R.S));
-    double l = L.sum_p * log_s;
+    double l = 0.0, mass = 0.0;
     for (int i = 0; i < A.parts; i++) {
-      const RowPart &r = s_part[i];
-      l += r.plogp - (r.ps + r.p * (static_cast<double>(r.ref()) - R.M)) / T_;
+      const RowPart &q = s_part[i];
+      l += q.plogp - (q.ps + q.p * (static_cast<double>(q.ref()) - R.M)) / T_;
+      mass += q.p;
     }
+    l += mass * log_s;
     if (L.rho != 0.0f)
       l += L.rho * (log(static_cast<double>(L.rho)) - log(static_cast<double>(R.S_off)) + log_s -
                     (static_cast<double>(R.M_off) - R.M) / T_);
@@ -480,88 +559,59 @@ __global__ void __launch_bounds__(kDistillThreads, 2) distill_kernel(const Disti
     A.loss[row] = static_cast<float>(static_cast<double>(w) * T_ * T_ * l);
     if (A.stats) A.stats[row] = make_float4(R.M, R.S, R.M_off, R.S_off);
   }
-  if constexpr (GRAD) {
-    const GradFactors g = grad_factors(L, R, A.c, by);
-    for (int b = 0; b < batches; b++) {
-      if (b > 0) load(b);
-#pragma unroll
-      for (int i = 0; i < kRes; i++) {
-        const int k = sp.k0 + (b * kRes + i) * NT + tid;
-        if (k < sp.k1) {
-          float x[N];
-          grad_vec<T>(raw[i], R.M_off, A.c, g.f, x);
-          store_row_vec<N>(g_row, A.V, sp.c0 + (k - sp.k0) * N, x, aligned);
-        }
-      }
-    }
-    __syncthreads();
-    grad_list(A, L, g_row, R.M, by, g.q_of_e, NT);
-  }
+  if constexpr (GRAD) write_gradient(A, L, sp, x_row, shift, g_row, aligned, R, __fmul_rn(w, A.T));
 }
 
-// The gradient from saved statistics: no sums are left to take, so a row's
-// tiles (256 threads x 8 vectors) are independent CTAs.
+// The gradient from saved statistics: no sums are left to take, so the parts
+// of a row are independent CTAs.
 template <typename T>
-__global__ void __launch_bounds__(kBackThreads) distill_backward_kernel(const DistillArgs A) {
-  constexpr int N = RowElem<T>::N;
-  constexpr int NT = kBackThreads;
-  __shared__ ListShared L;
-  __shared__ uint32_t s_bits[kRes * NT * N / 32];
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_backward_kernel(const DistillArgs A) {
+  extern __shared__ __align__(16) unsigned char s_dyn[];
   const int part = static_cast<int>(blockIdx.x) % A.parts;
   const int64_t row = blockIdx.x / A.parts;
-  const int tid = threadIdx.x;
   const T *x_row = static_cast<const T *>(A.logits) + row * A.ld;
   const int shift = row_shift(x_row);
   const Span<T> sp(part, A.span, A.V, shift);
   T *g_row = static_cast<T *>(A.grad) + row * A.ld_grad;
   const bool aligned = ((reinterpret_cast<uintptr_t>(g_row) - static_cast<uintptr_t>(shift) * sizeof(T)) & 15u) == 0;
   const float w = A.weight ? A.weight[row] : 1.0f;
-  if (w == 0.0f) {
-    zero_span(g_row, sp, A.V, aligned, NT);
-    return;
-  }
-  uint4 raw[kRes];
-#pragma unroll
-  for (int i = 0; i < kRes; i++) {
-    const int k = sp.k0 + i * NT + tid;
-    raw[i] = k < sp.k1 ? load_row_vec(x_row, shift, A.V, k) : make_uint4(0u, 0u, 0u, 0u);
-  }
+  const float up = A.grad_loss ? A.grad_loss[row] : 1.0f;
   const float4 st = A.stats[row];
-  const float by = __fmul_rn(__fmul_rn(w, A.T), A.grad_loss ? A.grad_loss[row] : 1.0f);
-  for (int i = tid; i < kRes * NT * N / 32; i += NT) s_bits[i] = 0u;
-  read_list(A, static_cast<int>(row), L);
-  __syncthreads();
-  if (!L.valid) {
-    zero_span(g_row, sp, A.V, aligned, NT);
+  bool target = w != 0.0f;
+  List L;
+  if (target) {
+    L = read_list(A, row, sp.c0, sp.c1, s_dyn, A.bit_words);
+    target = L.valid;
+  }
+  if (!target) {
+    zero_span(g_row, sp, A.V, aligned);
     return;
   }
-  mark_list(A, L, s_bits, x_row, sp.c0, sp.c1, NT);
-  __syncthreads();
-  join_doubles(A, L, NT);
-  const RowSums R{st.x, st.y, st.z, st.w};
-  const GradFactors g = grad_factors(L, R, A.c, by);
-#pragma unroll
-  for (int i = 0; i < kRes; i++) {
-    const int k = sp.k0 + i * NT + tid;
-    if (k < sp.k1) {
-      float x[N];
-      grad_vec<T>(raw[i], R.M_off, A.c, g.f, x);
-      store_row_vec<N>(g_row, A.V, sp.c0 + (k - sp.k0) * N, x, aligned);
-    }
-  }
-  __syncthreads();
-  grad_list(A, L, g_row, R.M, by, g.q_of_e, NT);
+  write_gradient(A, L, sp, x_row, shift, g_row, aligned, RowSums{st.x, st.y, st.z, st.w},
+                 __fmul_rn(__fmul_rn(w, A.T), up));
 }
 
-// CTAs per row: 64 KB of a row each; more, up to 8, while the rows would
-// leave SMs without a CTA.
+// The shared memory of a CTA: a bit per column of its span, and the list.
+template <typename T>
+size_t distill_smem(DistillArgs &A) {
+  A.bit_words = (A.span * RowElem<T>::N + 127) / 128 * 4;
+  return sizeof(uint32_t) * (static_cast<size_t>(A.bit_words) + 2 * static_cast<size_t>(A.K));
+}
+
+// CTAs per row.  The loss alone: whole rows while they fill the GPU's CTA
+// slots.  With the gradient: 64 KB of a row each, so that the rows in flight
+// stay in L2 for their second pass.  Either way more, up to 8, while the rows
+// would leave slots empty, and so many that a CTA's bits of its columns
+// stay within 24 KB (four CTAs share an SM).
 template <typename T, bool GRAD>
 cudaError_t launch_distill(DistillArgs &A, cudaStream_t st) {
   constexpr int N = RowElem<T>::N;
   const int vecs = (A.V + 2 * N - 2) / N;  // of a row with the largest shift
-  int parts = (vecs + kRes * kDistillThreads - 1) / (kRes * kDistillThreads);
-  while (parts < kMaxCluster && static_cast<int64_t>(A.N) * parts < 2 * current_sms() &&
-         vecs > parts * kDistillThreads)
+  int parts = GRAD ? (vecs + 4095) / 4096 : 1;
+  const int bits = (A.V + 24 * 1024 * 8 - 1) / (24 * 1024 * 8);
+  parts = parts > bits ? parts : bits;
+  while (parts < kMaxCluster && static_cast<int64_t>(A.N) * parts < kCtasPerSm * current_sms() &&
+         vecs > parts * kBatch * kThreads)
     parts++;
   parts = parts < kMaxCluster ? parts : kMaxCluster;
   A.parts = parts;
@@ -570,8 +620,8 @@ cudaError_t launch_distill(DistillArgs &A, cudaStream_t st) {
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(kDistillThreads);
-  cfg.dynamicSmemBytes = sizeof(uint32_t) * ((static_cast<size_t>(A.span) * N + 31) / 32);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = distill_smem<T>(A);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -584,15 +634,18 @@ cudaError_t launch_distill(DistillArgs &A, cudaStream_t st) {
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+// The gradient alone: parts of 64 KB.
 template <typename T>
 cudaError_t launch_backward(DistillArgs &A, cudaStream_t st) {
   constexpr int N = RowElem<T>::N;
   const int vecs = (A.V + 2 * N - 2) / N;
-  A.span = kRes * kBackThreads;
-  A.parts = (vecs + A.span - 1) / A.span;
+  A.parts = (vecs + 4095) / 4096;
+  while (static_cast<int64_t>(A.N) * A.parts < kCtasPerSm * current_sms() && vecs > A.parts * kThreads) A.parts *= 2;
+  A.span = (vecs + A.parts - 1) / A.parts;
   const int64_t ctas = static_cast<int64_t>(A.N) * A.parts;
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-  distill_backward_kernel<T><<<static_cast<unsigned>(ctas), kBackThreads, 0, st>>>(A);
+  const size_t smem = distill_smem<T>(A);
+  distill_backward_kernel<T><<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(A);
   return cudaGetLastError();
 }
 
