@@ -32,6 +32,8 @@
 // maximum and sums through distributed shared memory.  Columns beyond
 // 8 x 64 KB are read a second time (from L2, mostly: the rows in flight are
 // at most 148 x 2 / 8 of them).
+#include <atomic>
+
 #include "pz_device.cuh"
 #include "pz_rowvec.cuh"
 #include "pz_status.cuh"
@@ -44,6 +46,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;              // 16-byte vectors that a thread has in flight
 constexpr int kMaxCluster = 8;         // the portable cluster size
 constexpr int kCtasPerSm = 4;
+constexpr int kResident = 64 * 1024;   // most bytes of a row that a CTA keeps in shared memory
 
 struct DistillArgs {
   const void *logits;
@@ -65,6 +68,7 @@ struct DistillArgs {
   int parts;  // CTAs per row (the cluster's size in distill_kernel)
   int span;   // vectors per CTA
   int bit_words;  // words of a CTA's bits of listed columns, a multiple of 4
+  int resident;   // vectors of the span that stay in shared memory
 };
 
 // 2^x, fp32 results below 2^-126 flushed to zero (they are lost in any sum
@@ -78,10 +82,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // A CTA's view of its row's list, in shared memory; entry j belongs to thread
 // j % kThreads, which alone reads and writes it once the list is set up.
 struct List {
-  int32_t *id;     // [K]; -1: ignored, or a later entry of an id listed twice
-  float *p;        // [K] probabilities
   uint32_t *bits;  // one bit per column of the CTA's span: listed
-  double sum_p;
+  int32_t *id;     // [K]; -1: not in this CTA's columns, ignored, or a later entry of an id listed twice
+  float *p;        // [K] probabilities
+  float *log_p;    // [K]
+  float *s;        // [K] the student's logits
+  float mass;      // sum of p over the whole list, and rho
   float rho;
   bool valid;      // the row has a target
 };
@@ -101,97 +107,116 @@ struct Span {
   }
 };
 
-// Reads the row's list: ids and probabilities, their sum, rho, and the bits
-// of the ids in [c0, c1).  Two barriers of the block, the second one last.
-__device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, int c0, int c1, unsigned char *smem,
-                                          int bit_words) {
+// Reads the row's list: the probabilities and, of the ids in the CTA's
+// columns, bits and logits.  Two barriers of the block, the second one last.
+template <typename T, bool REST>
+__device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, const T *x_row, const Span<T> &sp,
+                                          unsigned char *smem) {
   __shared__ float s_top[kWarps];
   __shared__ int s_seen[kWarps], s_bad[kWarps];
   __shared__ double s_sum[kWarps];
   __shared__ int s_twice, s_gap;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int busy = min((A.K + 31) / 32, kWarps);  // warps with an entry
   List L;
   L.bits = reinterpret_cast<uint32_t *>(smem);
-  L.id = reinterpret_cast<int32_t *>(L.bits + bit_words);
+  L.id = reinterpret_cast<int32_t *>(L.bits + A.bit_words);
   L.p = reinterpret_cast<float *>(L.id + A.K);
-  const int32_t *ids = A.ids + row * A.ld_ids;
-  const float *values = A.values + row * A.ld_values;
-  const int n = A.n_list ? min(max(A.n_list[row], 0), A.K) : A.K;
+  L.log_p = L.p + A.K;
+  L.s = L.log_p + A.K;
   float top = -INFINITY;
   int seen = 0, bad = 0;
-  for (int j = tid; j < A.K; j += kThreads) {
-    int id = ids[j];
-    const float v = values[j];
-    float t = -INFINITY;
-    if (j >= n || id < 0 || id >= A.V) {
-      id = -1;
-    } else {
-      t = A.rest ? v : __fdiv_rn(v, A.T);
-      seen++;
-      bad |= t != t;
-      top = fmaxf(top, t);
+  if (warp < busy) {
+    const int32_t *ids = A.ids + row * A.ld_ids;
+    const float *values = A.values + row * A.ld_values;
+    const int n = A.n_list ? min(max(A.n_list[row], 0), A.K) : A.K;
+    for (int j = tid; j < A.K; j += kThreads) {
+      int id = ids[j];
+      float t = values[j];
+      if (j >= n || id < 0 || id >= A.V) {
+        id = -1;
+        t = -INFINITY;
+      } else {
+        if (!REST) t = __fdiv_rn(t, A.T);
+        seen++;
+        bad |= t != t;
+        top = fmaxf(top, t);
+      }
+      L.id[j] = id;
+      L.log_p[j] = t;
     }
-    L.id[j] = id;
-    L.p[j] = t;
-  }
-  for (int i = tid; i < bit_words / 4; i += kThreads) reinterpret_cast<uint4 *>(L.bits)[i] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  seen = __reduce_add_sync(0xFFFFFFFFu, seen);
-  bad = __any_sync(0xFFFFFFFFu, bad);
-  if (lane == 0) {
-    s_top[warp] = top;
-    s_seen[warp] = seen;
-    s_bad[warp] = bad;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    seen = __reduce_add_sync(0xFFFFFFFFu, seen);
+    bad = __any_sync(0xFFFFFFFFu, bad);
+    if (lane == 0) {
+      s_top[warp] = top;
+      s_seen[warp] = seen;
+      s_bad[warp] = bad;
+    }
   }
+  for (int i = tid; i < A.bit_words / 4; i += kThreads) reinterpret_cast<uint4 *>(L.bits)[i] = make_uint4(0u, 0u, 0u, 0u);
   if (tid == 0) s_twice = s_gap = 0;
   __syncthreads();
-  seen = 0;
-  for (int i = 0; i < kWarps; i++) {
+  top = -INFINITY;
+  seen = bad = 0;
+  for (int i = 0; i < busy; i++) {
     top = fmaxf(top, s_top[i]);
     seen += s_seen[i];
     bad |= s_bad[i];
   }
   // LIST: relative to the largest; REST: as they are
-  const float base = (A.rest || !(top > -INFINITY)) ? 0.0f : top;
-  double sum = 0.0;
-  for (int j = tid; j < A.K; j += kThreads) {
-    const int id = L.id[j];
-    const float p = id >= 0 ? expf(__fsub_rn(L.p[j], base)) : 0.0f;
-    L.p[j] = p;
-    sum += p;
-    if (id >= 0 && id >= c0 && id < c1) {
-      const uint32_t bit = 1u << ((id - c0) & 31);
-      if (atomicOr(&L.bits[(id - c0) >> 5], bit) & bit) s_twice = 1;
-    }
-  }
+  const float base = (REST || !(top > -INFINITY)) ? 0.0f : top;
   // A list that names every id leaves none for rho (what 1 - sum holds then
   // is rounding).
-  const bool whole = A.rest && seen >= A.V;
+  const bool whole = REST && seen >= A.V;
   if (whole) {
     for (int v = tid; v < A.V; v += kThreads) {
       bool on = false;
       for (int j = 0; j < A.K; j++) on |= L.id[j] == v;
       if (!on) s_gap = 1;
     }
+    __syncthreads();  // ids of other CTAs' columns leave the list below
   }
+  if (warp < busy) {
+    double sum = 0.0;
+    for (int j = tid; j < A.K; j += kThreads) {
+      const int id = L.id[j];
+      const float t = __fsub_rn(L.log_p[j], base);
+      const float p = id >= 0 ? expf(t) : 0.0f;
+      L.log_p[j] = t;
+      L.p[j] = p;
+      sum += p;
+      if (id >= 0 && id >= sp.c0 && id < sp.c1) {
+        const uint32_t bit = 1u << ((id - sp.c0) & 31);
+        L.s[j] = RowElem<T>::get(x_row + id);
+        if (atomicOr(&L.bits[(id - sp.c0) >> 5], bit) & bit) s_twice = 1;
+      } else {
+        L.id[j] = -1;
+      }
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  if (lane == 0) s_sum[warp] = sum;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+  }
   __syncthreads();
-  sum = 0.0;
-  for (int i = 0; i < kWarps; i++) sum += s_sum[i];
-  if (!A.rest) {
-    const float inv = static_cast<float>(1.0 / sum);
-    for (int j = tid; j < A.K; j += kThreads)
-      if (L.id[j] >= 0) L.p[j] = __fmul_rn(L.p[j], inv);
+  double sum = 0.0;
+  for (int i = 0; i < busy; i++) sum += s_sum[i];
+  if (!REST) {
+    if (warp < busy) {
+      const float inv = static_cast<float>(1.0 / sum), log_sum = logf(static_cast<float>(sum));
+      for (int j = tid; j < A.K; j += kThreads) {
+        L.p[j] = __fmul_rn(L.p[j], inv);
+        L.log_p[j] = __fsub_rn(L.log_p[j], log_sum);
+      }
+    }
     if (sum == sum) sum = 1.0;  // a NaN value makes the row's outputs NaN
   }
-  L.sum_p = sum;
-  // (an unordered comparison keeps a NaN sum: the row's outputs are NaN then)
-  L.rho = (A.rest && !(whole && !s_gap) && !(sum >= 1.0)) ? static_cast<float>(1.0 - sum) : 0.0f;
+  // (an unordered comparison keeps a NaN sum)
+  L.rho = (REST && !(whole && !s_gap) && !(sum >= 1.0)) ? static_cast<float>(1.0 - sum) : 0.0f;
+  L.mass = __fadd_rn(static_cast<float>(sum), L.rho);
   // no entries: no target.  LIST with no finite value: none either.
-  L.valid = seen > 0 && (A.rest || top > -INFINITY || bad);
+  L.valid = seen > 0 && (REST || top > -INFINITY || bad);
   if (s_twice) {
     // the first entry of an id takes the probabilities of all, in list order
     __syncthreads();
@@ -218,59 +243,102 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, int
       if (j < A.K) {
         if (joined[e] == -1.0f) L.id[j] = -1;
         L.p[j] = joined[e];
+        L.log_p[j] = logf(joined[e]);
       }
     }
   }
   return L;
 }
 
+// The row's columns as this thread sees them: vectors k0 + tid, k0 + tid +
+// kThreads, ... of the span.
 template <typename T>
-__device__ __forceinline__ void zero_span(T *row, const Span<T> &sp, int V, bool aligned) {
-  constexpr int N = RowElem<T>::N;
-  float x[N];
-#pragma unroll
-  for (int j = 0; j < N; j++) x[j] = 0.0f;
-  for (int k = sp.k0 + threadIdx.x; k < sp.k1; k += kThreads)
-    store_row_vec<N>(row, V, sp.c0 + (k - sp.k0) * N, x, aligned);
-}
+struct Columns {
+  static constexpr int N = RowElem<T>::N;
+  const T *row;
+  int V, shift;
+  WholeVecs whole;
+  Span<T> sp;
+  __device__ __forceinline__ Columns(const T *x_row, int V_, int part, int span)
+      : row(x_row), V(V_), shift(row_shift(x_row)), whole(whole_vecs<T>(shift, V_)), sp(part, span, V_, shift) {}
+  __device__ __forceinline__ bool in_one_piece(int k) const { return k >= whole.first && k < whole.last; }
+  __device__ __forceinline__ uint4 load(int k) const {
+    return in_one_piece(k) ? load16(row + (k * N - shift)) : load_edge(row, V, k * N - shift);
+  }
+  // Vector k into shared memory, asynchronously where it lies whole in the row.
+  __device__ __forceinline__ void fetch(uint4 *to, int k) const {
+    if (in_one_piece(k))
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                   "l"(row + (k * N - shift))
+                   : "memory");
+    else
+      *to = load_edge(row, V, k * N - shift);
+  }
+};
 
-// kBatch vectors of the span, from vector k on, kThreads apart.
+// The same columns of the gradient.
 template <typename T>
-__device__ __forceinline__ void load_batch(const T *row, int shift, int V, int k, int k1, uint4 *raw) {
+struct Gradient {
+  static constexpr int N = RowElem<T>::N;
+  T *row;
+  bool aligned;  // a vector of the logits is one of the gradient too
+  __device__ __forceinline__ Gradient(T *g_row, int shift)
+      : row(g_row),
+        aligned(((reinterpret_cast<uintptr_t>(g_row) - static_cast<uintptr_t>(shift) * sizeof(T)) & 15u) == 0) {}
+  __device__ __forceinline__ void store(const Columns<T> &C, int k, const float *x) const {
+    const int c = k * N - C.shift;
+    if (aligned && C.in_one_piece(k))
+      store16(row + c, RowElem<T>::pack(x));
+    else
+      store_edge<N>(row, C.V, c, x);
+  }
+  __device__ __forceinline__ void zero(const Columns<T> &C) const {
+    float x[N];
 #pragma unroll
-  for (int i = 0; i < kBatch; i++)
-    if (k + i * kThreads < k1) raw[i] = load_row_vec(row, shift, V, k + i * kThreads);
-}
+    for (int j = 0; j < N; j++) x[j] = 0.0f;
+    for (int k = C.sp.k0 + threadIdx.x; k < C.sp.k1; k += kThreads) store(C, k, x);
+  }
+};
 
 // A maximum and the sum of e relative to it.
 struct MaxSum {
   float m, s;
 };
-__device__ __forceinline__ MaxSum join(const MaxSum &a, const MaxSum &b, float c) {
-  MaxSum r;
-  r.m = fmaxf(a.m, b.m);
-  const float base = r.m > -INFINITY ? r.m : 0.0f;  // a side at -inf has s = 0 (or NaN, which stays)
-  r.s = __fadd_rn(__fmul_rn(a.s, exp2_approx(__fmul_rn(__fsub_rn(a.m, base), c))),
-                  __fmul_rn(b.s, exp2_approx(__fmul_rn(__fsub_rn(b.m, base), c))));
-  return r;
+__device__ __forceinline__ float exp_from(float x, float m, float c) {
+  return exp2_approx(__fmul_rn(__fsub_rn(x, m), c));
 }
-__device__ __forceinline__ MaxSum join_warp(MaxSum a, float c) {
+// The pairs of the lanes whose index differs in the bits of WIDTH - 1: their
+// maximum first, then each sum scaled once (a lane at -inf has the sum 0, or
+// NaN, which stays).
+template <int WIDTH>
+__device__ __forceinline__ MaxSum join_lanes(MaxSum a, float c) {
+  float m = a.m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const MaxSum b{__shfl_xor_sync(0xFFFFFFFFu, a.m, o), __shfl_xor_sync(0xFFFFFFFFu, a.s, o)};
-    a = join(a, b, c);
-  }
-  return a;
+  for (int o = WIDTH / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  float s = __fmul_rn(a.s, exp_from(a.m, m > -INFINITY ? m : 0.0f, c));
+#pragma unroll
+  for (int o = WIDTH / 2; o > 0; o >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xFFFFFFFFu, s, o));
+  return MaxSum{m, s};
+}
+__device__ __forceinline__ MaxSum join(const MaxSum &a, const MaxSum &b, float c) {
+  const float m = fmaxf(a.m, b.m), base = m > -INFINITY ? m : 0.0f;
+  return MaxSum{m, __fadd_rn(__fmul_rn(a.s, exp_from(a.m, base, c)), __fmul_rn(b.s, exp_from(b.m, base, c)))};
+}
+template <int WIDTH>
+__device__ __forceinline__ double sum_lanes(double x) {
+#pragma unroll
+  for (int o = WIDTH / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
+  return x;
 }
 
-// A CTA's part of its row's sums (warps hand in `row` and `list`).
+// A CTA's part of its row's sums.
 struct RowPart {
-  MaxSum row;          // its columns (REST: those off the list)
-  MaxSum list;         // REST: its listed ids
-  // over its listed ids: sum p, sum p log p, and sum p (s - ref), ref being
+  MaxSum row;   // its columns (REST: those off the list)
+  MaxSum list;  // REST: its listed ids
+  // over its listed ids: sum p, and sum p (log p - (s - ref) / T), ref being
   // the CTA's own maximum: the differences are taken before the sums, which
   // would lose them in rows of the type's lowest value
-  double p, plogp, ps, pad;
+  double p, l;
   __device__ __forceinline__ float ref() const {
     const float m = fmaxf(row.m, list.m);
     return m > -INFINITY ? m : 0.0f;
@@ -281,18 +349,17 @@ struct RowPart {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-// Copies *v to the same shared variable of CTA `rank` of the cluster.
+// Copies v to the same shared variable of CTA `rank` of the cluster.
 __device__ __forceinline__ void put_remote(const RowPart *slot, const RowPart &v, int rank) {
   uint32_t at;
   asm("mapa.shared::cluster.u32 %0, %1, %2;"
       : "=r"(at)
       : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(slot))), "r"(rank));
-  static_assert(sizeof(RowPart) == 48, "three 16-byte stores");
+  static_assert(sizeof(RowPart) == 32, "two 16-byte stores");
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.row.m), "f"(v.row.s), "f"(v.list.m),
                "f"(v.list.s)
                : "memory");
-  asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(at + 16), "d"(v.p), "d"(v.plogp) : "memory");
-  asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(at + 32), "d"(v.ps), "d"(v.pad) : "memory");
+  asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(at + 16), "d"(v.p), "d"(v.l) : "memory");
 }
 
 // The row's sums: M and S over all ids, M_off and S_off over those whose
@@ -301,104 +368,81 @@ struct RowSums {
   float M, S, M_off, S_off;
 };
 
-// What the passes multiply e by.
+// What the gradient multiplies e by.
 struct GradFactors {
+  float M, M_off;
   float q_of_e;  // listed ids, e relative to M: P / S
   float f;       // the others, e relative to M_off: w T (P / S 2^((M_off - M) c) - rho / S_off)
 };
 __device__ __forceinline__ GradFactors grad_factors(const List &L, const RowSums &R, float c, float by) {
   // a row without any weight (every logit -inf): its gradient is 0
-  if (R.S == 0.0f) return GradFactors{0.0f, 0.0f};
-  const float P = __fadd_rn(static_cast<float>(L.sum_p), L.rho);
-  GradFactors g;
-  g.q_of_e = __fdiv_rn(P, R.S);
+  if (R.S == 0.0f) return GradFactors{R.M, R.M_off, 0.0f, 0.0f};
+  GradFactors g{R.M, R.M_off, __fdiv_rn(L.mass, R.S), 0.0f};
   const float off = (L.rho == 0.0f || R.S_off == 0.0f) ? 0.0f : __fdiv_rn(L.rho, R.S_off);
-  const float q = __fmul_rn(g.q_of_e, exp2_approx(__fmul_rn(__fsub_rn(R.M_off, R.M), c)));
-  g.f = __fmul_rn(by, __fsub_rn(q, off));
+  g.f = __fmul_rn(by, __fsub_rn(__fmul_rn(g.q_of_e, exp_from(R.M_off, R.M, c)), off));
   return g;
 }
 
-// One batch of the pass along the row: e times f.
+// The gradient of the listed ids, over what the pass along the row wrote
+// there (a barrier before).
 template <typename T>
-__device__ __forceinline__ void grad_batch(const uint4 *raw, const Span<T> &sp, int k, int V, T *grad, bool aligned,
-                                           float m, float c, float f) {
-  constexpr int N = RowElem<T>::N;
-#pragma unroll
-  for (int i = 0; i < kBatch; i++) {
-    const int at = k + i * kThreads;
-    if (at < sp.k1) {
-      float x[N];
-      RowElem<T>::unpack(raw[i], x);
-#pragma unroll
-      for (int j = 0; j < N; j++) x[j] = __fmul_rn(exp2_approx(__fmul_rn(__fsub_rn(x[j], m), c)), f);
-      store_row_vec<N>(grad, V, sp.c0 + (at - sp.k0) * N, x, aligned);
-    }
+__device__ __forceinline__ void grad_list(const DistillArgs &A, const List &L, const GradFactors &g, T *grad, float by) {
+  for (int j = threadIdx.x; j < A.K; j += kThreads) {
+    const int id = L.id[j];
+    if (id < 0) continue;
+    const float e = exp_from(L.s[j], g.M, A.c);
+    RowElem<T>::put(grad + id, g.q_of_e == 0.0f ? 0.0f : __fmul_rn(by, __fsub_rn(__fmul_rn(e, g.q_of_e), L.p[j])));
   }
 }
 
-// The pass along the row, the next batch in flight while one is worked on;
-// then the listed ids get their own gradient over what the pass wrote there.
-// Their logits are read before it: the gradient may lie over the logits.
 template <typename T>
-__device__ __forceinline__ void write_gradient(const DistillArgs &A, const List &L, const Span<T> &sp, const T *row,
-                                               int shift, T *grad, bool aligned, const RowSums &R, float by) {
-  constexpr int STEP = kBatch * kThreads;
-  const GradFactors g = grad_factors(L, R, A.c, by);
-  constexpr int E = PZ_TOP_K_MAX / kThreads;
-  float own[E];
+__device__ __forceinline__ void grad_vec(const uint4 &raw, float m, float c, float f, float *x) {
+  RowElem<T>::unpack(raw, x);
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int j = static_cast<int>(threadIdx.x) + e * kThreads;
-    own[e] = 0.0f;
-    if (j < A.K) {
-      const int id = L.id[j];
-      if (id >= 0 && id >= sp.c0 && id < sp.c1) own[e] = RowElem<T>::get(row + id);
+  for (int j = 0; j < RowElem<T>::N; j++) x[j] = __fmul_rn(exp_from(x[j], m, c), f);
+}
+
+// The vectors from `k` on, straight from global memory, the next batch in
+// flight while one is worked on.
+template <typename T>
+__device__ __forceinline__ void grad_stream(const Columns<T> &C, const Gradient<T> &G, const GradFactors &g, float c,
+                                            int k) {
+  uint4 now[kBatch], next[kBatch];
+#pragma unroll
+  for (int i = 0; i < kBatch; i++)
+    if (k + i * kThreads < C.sp.k1) now[i] = C.load(k + i * kThreads);
+  while (k < C.sp.k1) {
+    const int ahead = k + kBatch * kThreads;
+#pragma unroll
+    for (int i = 0; i < kBatch; i++)
+      if (ahead + i * kThreads < C.sp.k1) next[i] = C.load(ahead + i * kThreads);
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      if (k + i * kThreads < C.sp.k1) {
+        float x[RowElem<T>::N];
+        grad_vec<T>(now[i], g.M_off, c, g.f, x);
+        G.store(C, k + i * kThreads, x);
+      }
+      now[i] = next[i];
     }
-  }
-  int k = sp.k0 + static_cast<int>(threadIdx.x);
-  uint4 a[kBatch], b[kBatch];
-  load_batch(row, shift, A.V, k, sp.k1, a);
-  // every listed logit of the span has been read (their values are used
-  // below, behind this barrier's wait for the loads)
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const float x = exp2_approx(__fmul_rn(__fsub_rn(own[e], R.M), A.c));
-    own[e] = __fmul_rn(x, g.q_of_e);
-  }
-  __syncthreads();
-  for (; k < sp.k1; k += 2 * STEP) {
-    load_batch(row, shift, A.V, k + STEP, sp.k1, b);
-    grad_batch(a, sp, k, A.V, grad, aligned, R.M_off, A.c, g.f);
-    load_batch(row, shift, A.V, k + 2 * STEP, sp.k1, a);
-    grad_batch(b, sp, k + STEP, A.V, grad, aligned, R.M_off, A.c, g.f);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int j = static_cast<int>(threadIdx.x) + e * kThreads;
-    if (j < A.K) {
-      const int id = L.id[j];
-      if (id >= 0 && id >= sp.c0 && id < sp.c1)
-        RowElem<T>::put(grad + id, g.q_of_e == 0.0f ? 0.0f : __fmul_rn(by, __fsub_rn(own[e], L.p[j])));
-    }
+    k = ahead;
   }
 }
 
 // One batch into a thread's running maximum and sum.  REST: listed ids are
 // left out.
-template <typename T>
-__device__ __forceinline__ void sum_batch(const DistillArgs &A, const List &L, const Span<T> &sp, uint4 *raw, int k,
-                                          MaxSum &a) {
+template <typename T, bool REST>
+__device__ __forceinline__ void sum_batch(const List &L, const Columns<T> &C, float c, uint4 *raw, int k, MaxSum &a) {
   constexpr int N = RowElem<T>::N;
   float x[N];
   float top = a.m;
 #pragma unroll
   for (int i = 0; i < kBatch; i++) {
     const int at = k + i * kThreads;
-    if (at >= sp.k1) {
+    if (at >= C.sp.k1) {
       raw[i] = make_uint4(RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2);
-    } else if (A.rest) {
-      const int u = (at - sp.k0) * N;
+    } else if (REST) {
+      const int u = (at - C.sp.k0) * N;
       const uint32_t on = (L.bits[u >> 5] >> (u & 31)) & ((1u << N) - 1u);
       if (on != 0u) {
         RowElem<T>::unpack(raw[i], x);
@@ -408,49 +452,50 @@ __device__ __forceinline__ void sum_batch(const DistillArgs &A, const List &L, c
         raw[i] = RowElem<T>::pack(x);
       }
     }
-    RowElem<T>::unpack(raw[i], x);
-#pragma unroll
-    for (int j = 0; j < N; j++) top = fmaxf(top, x[j]);
+    top = fmaxf(top, RowElem<T>::max(raw[i]));
   }
   const float base = top > -INFINITY ? top : 0.0f;
-  float s = __fmul_rn(a.s, exp2_approx(__fmul_rn(__fsub_rn(a.m, base), A.c)));
+  float s = __fmul_rn(a.s, exp_from(a.m, base, c));
 #pragma unroll
   for (int i = 0; i < kBatch; i++) {
     RowElem<T>::unpack(raw[i], x);
 #pragma unroll
-    for (int j = 0; j < N; j++) s = __fadd_rn(s, exp2_approx(__fmul_rn(__fsub_rn(x[j], base), A.c)));
+    for (int j = 0; j < N; j++) s = __fadd_rn(s, exp_from(x[j], base, c));
   }
   a = MaxSum{top, s};
 }
 
-template <typename T, bool GRAD>
+template <typename T, bool REST, bool GRAD>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const DistillArgs A) {
   constexpr int STEP = kBatch * kThreads;
   __shared__ __align__(16) RowPart s_part[kMaxCluster];
   __shared__ MaxSum s_warp[kWarps][2];
+  __shared__ double s_list[kWarps][2];
+  __shared__ GradFactors s_factors;
   extern __shared__ __align__(16) unsigned char s_dyn[];
   const int part = static_cast<int>(blockIdx.x) % A.parts;
   const int64_t row = blockIdx.x / A.parts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const T *x_row = static_cast<const T *>(A.logits) + row * A.ld;
-  const int shift = row_shift(x_row);
-  const Span<T> sp(part, A.span, A.V, shift);
-  T *g_row = GRAD ? static_cast<T *>(A.grad) + row * A.ld_grad : nullptr;
-  const bool aligned =
-      GRAD && ((reinterpret_cast<uintptr_t>(g_row) - static_cast<uintptr_t>(shift) * sizeof(T)) & 15u) == 0;
+  const Columns<T> C(static_cast<const T *>(A.logits) + row * A.ld, A.V, part, A.span);
   const float w = A.weight ? A.weight[row] : 1.0f;
+  const float by = __fmul_rn(w, A.T);
 
   bool target = w != 0.0f;
   List L;
-  uint4 ra[kBatch], rb[kBatch];
-  int k = sp.k0 + tid;
+  uint4 *held = reinterpret_cast<uint4 *>(s_dyn);
+  const int k_held = GRAD ? min(C.sp.k0 + A.resident, C.sp.k1) : C.sp.k0;  // the vectors before stay on chip
   if (target) {
-    load_batch(x_row, shift, A.V, k, sp.k1, ra);
-    L = read_list(A, row, sp.c0, sp.c1, s_dyn, A.bit_words);
+    if (GRAD) {
+      for (int k = C.sp.k0 + tid; k < k_held; k += kThreads) C.fetch(held + (k - C.sp.k0), k);
+    }
+    L = read_list<T, REST>(A, row, C.row, C.sp, s_dyn + static_cast<size_t>(A.resident) * 16);
     target = L.valid;
   }
   if (!target) {  // the whole cluster leaves
-    if (GRAD) zero_span(g_row, sp, A.V, aligned);
+    if (GRAD) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      Gradient<T>(static_cast<T *>(A.grad) + row * A.ld_grad, C.shift).zero(C);
+    }
     if (part == 0 && tid == 0) {
       A.loss[row] = 0.0f;
       if (A.stats) A.stats[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -461,153 +506,175 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
 
   // running maximum and sum of this thread's columns
   MaxSum a{-INFINITY, 0.0f};
-  for (; k < sp.k1; k += 2 * STEP) {
-    load_batch(x_row, shift, A.V, k + STEP, sp.k1, rb);
-    sum_batch(A, L, sp, ra, k, a);
-    load_batch(x_row, shift, A.V, k + 2 * STEP, sp.k1, ra);
-    if (k + STEP < sp.k1) sum_batch(A, L, sp, rb, k + STEP, a);
+  {
+    uint4 now[kBatch], next[kBatch];
+    int k = k_held + tid;
+#pragma unroll
+    for (int i = 0; i < kBatch; i++)
+      if (k + i * kThreads < C.sp.k1) now[i] = C.load(k + i * kThreads);
+    while (k < C.sp.k1) {
+#pragma unroll
+      for (int i = 0; i < kBatch; i++)
+        if (k + STEP + i * kThreads < C.sp.k1) next[i] = C.load(k + STEP + i * kThreads);
+      sum_batch<T, REST>(L, C, A.c, now, k, a);
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) now[i] = next[i];
+      k += STEP;
+    }
   }
+  if (GRAD) {
+    asm volatile("cp.async.wait_all;" ::: "memory");  // a thread reads back what it fetched itself
+    Columns<T> H = C;
+    H.sp.k1 = k_held;
+    for (int k = C.sp.k0 + tid; k < k_held; k += STEP) {
+      uint4 now[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; i++)
+        if (k + i * kThreads < k_held) now[i] = held[k + i * kThreads - C.sp.k0];
+      sum_batch<T, REST>(L, H, A.c, now, k, a);
+    }
+  }
+  a = join_lanes<32>(a, A.c);
   // and of its listed ids
-  MaxSum listed{-INFINITY, 0.0f};
-  if (A.rest) {
-    for (int j = tid; j < A.K; j += kThreads) {
-      const int id = L.id[j];
-      if (id < 0 || id < sp.c0 || id >= sp.c1) continue;
-      const float sv = RowElem<T>::get(x_row + id);
-      listed = join(listed, MaxSum{sv, sv == -INFINITY ? 0.0f : 1.0f}, A.c);
-    }
-    listed = join_warp(listed, A.c);
+  const int busy = min((A.K + 31) / 32, kWarps);
+  if (REST && warp < busy) {
+    MaxSum listed{-INFINITY, 0.0f};
+    for (int j = tid; j < A.K; j += kThreads)
+      if (L.id[j] >= 0) listed = join(listed, MaxSum{L.s[j], L.s[j] == -INFINITY ? 0.0f : 1.0f}, A.c);
+    listed = join_lanes<32>(listed, A.c);
+    if (lane == 0) s_warp[warp][1] = listed;
   }
-  a = join_warp(a, A.c);
-  if (lane == 0) {
-    s_warp[warp][0] = a;
-    s_warp[warp][1] = listed;
-  }
+  if (lane == 0) s_warp[warp][0] = a;
   __syncthreads();
-  RowPart r{s_warp[0][0], s_warp[0][1], 0.0, 0.0, 0.0, 0.0};
-  for (int i = 1; i < kWarps; i++) {
-    r.row = join(r.row, s_warp[i][0], A.c);
-    r.list = join(r.list, s_warp[i][1], A.c);
-  }
-  const double ref = r.ref();
-  for (int j = tid; j < A.K; j += kThreads) {
-    const int id = L.id[j];
-    const float p = L.p[j];
-    if (id < 0 || id < sp.c0 || id >= sp.c1 || p == 0.0f) continue;
-    r.p += p;
-    r.plogp += static_cast<double>(p) * logf(p);
-    r.ps += static_cast<double>(p) * (RowElem<T>::get(x_row + id) - ref);
-  }
-  if (A.K > 32) {  // entries in several warps
-    __shared__ double s_list[kWarps][3];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      r.p += __shfl_xor_sync(0xFFFFFFFFu, r.p, o);
-      r.plogp += __shfl_xor_sync(0xFFFFFFFFu, r.plogp, o);
-      r.ps += __shfl_xor_sync(0xFFFFFFFFu, r.ps, o);
+  if (warp < busy) {
+    RowPart r;
+    r.row = join_lanes<kWarps>(s_warp[lane & (kWarps - 1)][0], A.c);
+    r.list = MaxSum{-INFINITY, 0.0f};
+    if (REST) r.list = join_lanes<kWarps>((lane & (kWarps - 1)) < busy ? s_warp[lane & (kWarps - 1)][1] : r.list, A.c);
+    const double ref = r.ref(), inv_T = 1.0 / static_cast<double>(A.T);
+    r.p = r.l = 0.0;
+    for (int j = tid; j < A.K; j += kThreads) {
+      const float p = L.p[j];
+      if (L.id[j] < 0 || p == 0.0f) continue;
+      r.p += p;
+      r.l += p * (L.log_p[j] - (L.s[j] - ref) * inv_T);
     }
-    if (lane == 0) {
-      s_list[warp][0] = r.p;
-      s_list[warp][1] = r.plogp;
-      s_list[warp][2] = r.ps;
+    r.p = sum_lanes<32>(r.p);
+    r.l = sum_lanes<32>(r.l);
+    if (busy > 1) {
+      if (lane == 0) {
+        s_list[warp][0] = r.p;
+        s_list[warp][1] = r.l;
+      }
+      asm volatile("bar.sync 1, %0;" ::"r"(32 * busy) : "memory");  // of the warps with an entry
+      r.p = r.l = 0.0;
+      for (int i = 0; i < busy; i++) {
+        r.p += s_list[i][0];
+        r.l += s_list[i][1];
+      }
     }
-    __syncthreads();
-    r.p = r.plogp = r.ps = 0.0;
-    for (int i = 0; i < kWarps; i++) {
-      r.p += s_list[i][0];
-      r.plogp += s_list[i][1];
-      r.ps += s_list[i][2];
-    }
-  } else if (warp == 0) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      r.p += __shfl_xor_sync(0xFFFFFFFFu, r.p, o);
-      r.plogp += __shfl_xor_sync(0xFFFFFFFFu, r.plogp, o);
-      r.ps += __shfl_xor_sync(0xFFFFFFFFu, r.ps, o);
+    if (warp == 0) {
+      cluster_wait();  // every CTA of the row runs: its shared memory may be written
+      if (lane < A.parts) put_remote(&s_part[part], r, lane);
     }
   }
-  cluster_wait();  // every CTA of the row runs: its shared memory may be written
-  if (tid < A.parts) put_remote(&s_part[part], r, tid);
+  if (warp != 0) cluster_wait();
   cluster_arrive();
   cluster_wait();
-  RowPart all = s_part[0];
-  for (int i = 1; i < A.parts; i++) {
-    all.row = join(all.row, s_part[i].row, A.c);
-    all.list = join(all.list, s_part[i].list, A.c);
-  }
-  RowSums R{all.row.m, all.row.s, all.row.m, all.row.s};
-  if (A.rest) {
-    const MaxSum both = join(all.row, all.list, A.c);
-    R.M = both.m;
-    R.S = both.s;
-  }
-  if (!(R.M > -INFINITY)) R.M = 0.0f;
-  if (!(R.M_off > -INFINITY)) R.M_off = R.M;
-  if (part == 0 && tid == 0) {
-    const double T_ = A.T, log_s = log(static_cast<double>(R.S));
-    double l = 0.0, mass = 0.0;
-    for (int i = 0; i < A.parts; i++) {
-      const RowPart &q = s_part[i];
-      l += q.plogp - (q.ps + q.p * (static_cast<double>(q.ref()) - R.M)) / T_;
-      mass += q.p;
+  if (warp == 0) {
+    const RowPart none{{-INFINITY, 0.0f}, {-INFINITY, 0.0f}, 0.0, 0.0};
+    const RowPart mine = lane < A.parts ? s_part[lane] : none;
+    const MaxSum all = join_lanes<kMaxCluster>(mine.row, A.c);
+    RowSums R{all.m, all.s, all.m, all.s};
+    if (REST) {
+      const MaxSum both = join(all, join_lanes<kMaxCluster>(mine.list, A.c), A.c);
+      R.M = both.m;
+      R.S = both.s;
     }
-    l += mass * log_s;
-    if (L.rho != 0.0f)
-      l += L.rho * (log(static_cast<double>(L.rho)) - log(static_cast<double>(R.S_off)) + log_s -
-                    (static_cast<double>(R.M_off) - R.M) / T_);
-    if (R.S == 0.0f) l = INFINITY;  // every logit is -inf: the student has no distribution
-    A.loss[row] = static_cast<float>(static_cast<double>(w) * T_ * T_ * l);
-    if (A.stats) A.stats[row] = make_float4(R.M, R.S, R.M_off, R.S_off);
+    if (!(R.M > -INFINITY)) R.M = 0.0f;
+    if (!(R.M_off > -INFINITY)) R.M_off = R.M;
+    if (GRAD && lane == 0) s_factors = grad_factors(L, R, A.c, by);
+    if (part == 0) {
+      const double T_ = A.T;
+      const double mass = sum_lanes<kMaxCluster>(mine.p);
+      double l = sum_lanes<kMaxCluster>(mine.l - mine.p * ((static_cast<double>(mine.ref()) - R.M) / T_));
+      if (lane == 0) {
+        const double log_s = log(static_cast<double>(R.S));
+        l += mass * log_s;
+        if (L.rho != 0.0f)
+          l += L.rho * (log(static_cast<double>(L.rho) / R.S_off) + log_s - (static_cast<double>(R.M_off) - R.M) / T_);
+        if (R.S == 0.0f) l = INFINITY;  // every logit is -inf: the student has no distribution
+        A.loss[row] = static_cast<float>(static_cast<double>(w) * T_ * T_ * l);
+        if (A.stats) A.stats[row] = make_float4(R.M, R.S, R.M_off, R.S_off);
+      }
+    }
   }
-  if constexpr (GRAD) write_gradient(A, L, sp, x_row, shift, g_row, aligned, R, __fmul_rn(w, A.T));
+  if constexpr (GRAD) {
+    __syncthreads();
+    const GradFactors g = s_factors;
+    const Gradient<T> G(static_cast<T *>(A.grad) + row * A.ld_grad, C.shift);
+#pragma unroll 2
+    for (int k = C.sp.k0 + tid; k < k_held; k += kThreads) {
+      float x[RowElem<T>::N];
+      grad_vec<T>(held[k - C.sp.k0], g.M_off, A.c, g.f, x);
+      G.store(C, k, x);
+    }
+    if (k_held < C.sp.k1) grad_stream(C, G, g, A.c, k_held + tid);
+    __syncthreads();
+    grad_list(A, L, g, G.row, by);
+  }
 }
 
 // The gradient from saved statistics: no sums are left to take, so the parts
 // of a row are independent CTAs.
-template <typename T>
+template <typename T, bool REST>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_backward_kernel(const DistillArgs A) {
   extern __shared__ __align__(16) unsigned char s_dyn[];
   const int part = static_cast<int>(blockIdx.x) % A.parts;
   const int64_t row = blockIdx.x / A.parts;
-  const T *x_row = static_cast<const T *>(A.logits) + row * A.ld;
-  const int shift = row_shift(x_row);
-  const Span<T> sp(part, A.span, A.V, shift);
-  T *g_row = static_cast<T *>(A.grad) + row * A.ld_grad;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(g_row) - static_cast<uintptr_t>(shift) * sizeof(T)) & 15u) == 0;
+  const Columns<T> C(static_cast<const T *>(A.logits) + row * A.ld, A.V, part, A.span);
+  const Gradient<T> G(static_cast<T *>(A.grad) + row * A.ld_grad, C.shift);
   const float w = A.weight ? A.weight[row] : 1.0f;
   const float up = A.grad_loss ? A.grad_loss[row] : 1.0f;
   const float4 st = A.stats[row];
   bool target = w != 0.0f;
   List L;
   if (target) {
-    L = read_list(A, row, sp.c0, sp.c1, s_dyn, A.bit_words);
+    L = read_list<T, REST>(A, row, C.row, C.sp, s_dyn);
     target = L.valid;
   }
   if (!target) {
-    zero_span(g_row, sp, A.V, aligned);
+    G.zero(C);
     return;
   }
-  write_gradient(A, L, sp, x_row, shift, g_row, aligned, RowSums{st.x, st.y, st.z, st.w},
-                 __fmul_rn(__fmul_rn(w, A.T), up));
+  const float by = __fmul_rn(__fmul_rn(w, A.T), up);
+  const GradFactors g = grad_factors(L, RowSums{st.x, st.y, st.z, st.w}, A.c, by);
+  // (read_list has read the listed logits: the gradient may lie over them)
+  grad_stream(C, G, g, A.c, C.sp.k0 + static_cast<int>(threadIdx.x));
+  __syncthreads();
+  grad_list(A, L, g, G.row, by);
 }
 
-// The shared memory of a CTA: a bit per column of its span, and the list.
+// The shared memory of a CTA: the resident vectors, a bit per column of its
+// span, and the list.
 template <typename T>
 size_t distill_smem(DistillArgs &A) {
   A.bit_words = (A.span * RowElem<T>::N + 127) / 128 * 4;
-  return sizeof(uint32_t) * (static_cast<size_t>(A.bit_words) + 2 * static_cast<size_t>(A.K));
+  return static_cast<size_t>(A.resident) * 16 +
+         sizeof(uint32_t) * (static_cast<size_t>(A.bit_words) + 4 * static_cast<size_t>(A.K));
 }
 
 // CTAs per row.  The loss alone: whole rows while they fill the GPU's CTA
-// slots.  With the gradient: 64 KB of a row each, so that the rows in flight
-// stay in L2 for their second pass.  Either way more, up to 8, while the rows
-// would leave slots empty, and so many that a CTA's bits of its columns
-// stay within 24 KB (four CTAs share an SM).
-template <typename T, bool GRAD>
-cudaError_t launch_distill(DistillArgs &A, cudaStream_t st) {
+// slots.  With the gradient: 32 KB of a row each, which with four CTAs per SM
+// stay in shared memory between the two passes; a row of more than 8 x 64 KB
+// is read a second time beyond that.  Either way more CTAs, up to 8, while
+// the rows would leave slots empty, and so many that a CTA's bits of its
+// columns stay within 24 KB.
+template <typename T, bool REST, bool GRAD>
+cudaError_t launch_distill_as(DistillArgs &A, cudaStream_t st) {
   constexpr int N = RowElem<T>::N;
   const int vecs = (A.V + 2 * N - 2) / N;  // of a row with the largest shift
-  int parts = GRAD ? (vecs + 4095) / 4096 : 1;
+  int parts = GRAD ? (vecs + 2047) / 2048 : 1;
   const int bits = (A.V + 24 * 1024 * 8 - 1) / (24 * 1024 * 8);
   parts = parts > bits ? parts : bits;
   while (parts < kMaxCluster && static_cast<int64_t>(A.N) * parts < kCtasPerSm * current_sms() &&
@@ -616,12 +683,17 @@ cudaError_t launch_distill(DistillArgs &A, cudaStream_t st) {
   parts = parts < kMaxCluster ? parts : kMaxCluster;
   A.parts = parts;
   A.span = (vecs + parts - 1) / parts;
+  A.resident = GRAD ? (A.span < kResident / 16 ? A.span : kResident / 16) : 0;
   const int64_t ctas = static_cast<int64_t>(A.N) * parts;
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+  const size_t smem = distill_smem<T>(A);
+  static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+  cudaError_t e = allow_smem(reinterpret_cast<const void *>(distill_kernel<T, REST, GRAD>), 112 * 1024, &ready);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = distill_smem<T>(A);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -630,11 +702,19 @@ cudaError_t launch_distill(DistillArgs &A, cudaStream_t st) {
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_kernel<T, GRAD>, A);
+  e = cudaLaunchKernelEx(&cfg, distill_kernel<T, REST, GRAD>, A);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-// The gradient alone: parts of 64 KB.
+template <bool GRAD>
+cudaError_t launch_distill(DistillArgs &A, pz_dtype dtype, cudaStream_t st) {
+  if (dtype == PZ_DTYPE_F32)
+    return A.rest ? launch_distill_as<float, true, GRAD>(A, st) : launch_distill_as<float, false, GRAD>(A, st);
+  return A.rest ? launch_distill_as<bf16_t, true, GRAD>(A, st) : launch_distill_as<bf16_t, false, GRAD>(A, st);
+}
+
+// The gradient alone: parts of 64 KB, smaller ones while the rows would leave
+// SMs without a CTA.
 template <typename T>
 cudaError_t launch_backward(DistillArgs &A, cudaStream_t st) {
   constexpr int N = RowElem<T>::N;
@@ -645,7 +725,10 @@ cudaError_t launch_backward(DistillArgs &A, cudaStream_t st) {
   const int64_t ctas = static_cast<int64_t>(A.N) * A.parts;
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
   const size_t smem = distill_smem<T>(A);
-  distill_backward_kernel<T><<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(A);
+  if (A.rest)
+    distill_backward_kernel<T, true><<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(A);
+  else
+    distill_backward_kernel<T, false><<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(A);
   return cudaGetLastError();
 }
 
@@ -716,8 +799,7 @@ pz_status pz_distill_forward(const void *logits, pz_dtype dtype, int N, int V, i
   A.loss = loss;
   A.stats = reinterpret_cast<float4 *>(stats);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == PZ_DTYPE_F32 ? pz::launch_distill<float, false>(A, st)
-                                              : pz::launch_distill<pz::bf16_t, false>(A, st);
+  const cudaError_t e = pz::launch_distill<false>(A, dtype, st);
   return e == cudaSuccess ? PZ_OK : pz::report_cuda(e);
 }
 
@@ -752,8 +834,7 @@ pz_status pz_distill_loss_grad(const void *logits, pz_dtype dtype, int N, int V,
   if (s != PZ_OK || N == 0) return s;
   A.loss = loss;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == PZ_DTYPE_F32 ? pz::launch_distill<float, true>(A, st)
-                                              : pz::launch_distill<pz::bf16_t, true>(A, st);
+  const cudaError_t e = pz::launch_distill<true>(A, dtype, st);
   return e == cudaSuccess ? PZ_OK : pz::report_cuda(e);
 }
 

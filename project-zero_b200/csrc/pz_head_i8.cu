@@ -409,14 +409,8 @@ cudaError_t launch_matmul_as(const MatmulArgs &P, bool after_quantize, cudaStrea
     return cudaErrorInvalidValue;
   const size_t smem = static_cast<size_t>(A.stages) * stage + 1024;
   static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = allow_smem(reinterpret_cast<const void *>(matmul_i8_kernel<T>), kTcRing + 1024, &ready);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !((ready.load(std::memory_order_acquire) >> dev) & 1u)) {
-    e = cudaFuncSetAttribute(matmul_i8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcRing + 1024);
-    if (e != cudaSuccess) return e;
-    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
-  }
   cudaLaunchConfig_t cfg{};
   const int sms = current_sms();
   cfg.gridDim = dim3(static_cast<unsigned>(A.tiles < sms ? A.tiles : sms));

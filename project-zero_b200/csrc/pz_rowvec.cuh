@@ -34,6 +34,9 @@ struct RowElem<float> {
   static __device__ __forceinline__ uint4 pack(const float *x) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
   }
+  static __device__ __forceinline__ float max(const uint4 &u) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
   static constexpr uint32_t kNegInf2 = 0xFF800000u;  // what a 32-bit word of -inf holds
 };
 
@@ -62,6 +65,12 @@ struct RowElem<bf16_t> {
   static __device__ __forceinline__ uint4 pack(const float *x) {
     return make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
   }
+  // the largest value that is not NaN (NaN where all are), two at a time
+  static __device__ __forceinline__ float max(const uint4 &u) {
+    const __nv_bfloat162 *v = reinterpret_cast<const __nv_bfloat162 *>(&u);
+    const __nv_bfloat162 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
   static constexpr uint32_t kNegInf2 = 0xFF80FF80u;
 };
 
@@ -82,6 +91,33 @@ __device__ __forceinline__ uint4 load16(const void *p) {
 }
 __device__ __forceinline__ void store16(void *p, const uint4 &v) {
   __stcs(reinterpret_cast<uint4 *>(p), v);
+}
+
+// Vectors [first, last) of a row lie in it whole.
+struct WholeVecs {
+  int first, last;
+};
+template <typename T>
+__device__ __forceinline__ WholeVecs whole_vecs(int shift, int V) {
+  return WholeVecs{shift > 0 ? 1 : 0, (V + shift) / RowElem<T>::N};
+}
+
+// Columns [c, c + N) that reach outside the row, those outside as -inf.  Out
+// of line: at most two vectors of a row take this way.
+template <typename T>
+__device__ __noinline__ uint4 load_edge(const T *row, int V, int c) {
+  constexpr int N = RowElem<T>::N;
+  float x[N];
+#pragma unroll
+  for (int j = 0; j < N; j++)
+    x[j] = (c + j >= 0 && c + j < V) ? RowElem<T>::get(row + c + j) : __int_as_float(0xFF800000);
+  return RowElem<T>::pack(x);
+}
+// Columns [c, c + N) of a row, those inside [0, V), one at a time.
+template <int N, typename T>
+__device__ __noinline__ void store_edge(T *row, int V, int c, const float *x) {
+  for (int j = 0; j < N; j++)
+    if (c + j >= 0 && c + j < V) RowElem<T>::put(row + c + j, x[j]);
 }
 
 // Vector k of the row: packed, columns outside [0, V) as -inf.

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/pz_sampling.h"
 
 namespace pz {
@@ -16,6 +18,18 @@ pz_status report_cuda(cudaError_t e);
 // SMs of the current device, looked up once per device (148 where the
 // lookup fails).
 int current_sms();
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device,
+// once per device (`ready`: a bit per device, the kernel's own).
+inline cudaError_t allow_smem(const void *kernel, int bytes, std::atomic<uint64_t> *ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && ((ready->load(std::memory_order_acquire) >> dev) & 1u)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) ready->fetch_or(1ull << dev, std::memory_order_release);
+  return e;
+}
 
 // Bytes of B rows of V elements, `ld` elements apart.
 inline uint64_t rows_bytes(int B, int V, int64_t ld, size_t es) {
