@@ -43,7 +43,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBatch = 4;              // 16-byte vectors that a thread has in flight
+constexpr int kBatch = 4;              // 16-byte vectors that a thread works on at a time
+constexpr int kStep = kBatch * kThreads;
+constexpr int kEntries = PZ_TOP_K_MAX / kThreads;  // most list entries of a thread
+constexpr int kFlagWords = 2;
+constexpr int kMaxSpan = kFlagWords * 32 * kStep;   // vectors of a span: a flag per batch of a thread
 constexpr int kMaxCluster = 8;         // the portable cluster size
 constexpr int kCtasPerSm = 4;
 constexpr int kResident = 64 * 1024;   // most bytes of a row that a CTA keeps in shared memory
@@ -60,6 +64,7 @@ struct DistillArgs {
   const float *weight;
   const float *grad_loss;
   float T, c;
+  double inv_T;
   int rest;
   float *loss;
   float4 *stats;
@@ -83,6 +88,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // j % kThreads, which alone reads and writes it once the list is set up.
 struct List {
   uint32_t *bits;  // one bit per column of the CTA's span: listed
+  uint32_t flags[kFlagWords];  // this thread's batches that hold a listed column
   int32_t *id;     // [K]; -1: not in this CTA's columns, ignored, or a later entry of an id listed twice
   float *p;        // [K] probabilities
   float *log_p;    // [K]
@@ -116,6 +122,7 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
   __shared__ int s_seen[kWarps], s_bad[kWarps];
   __shared__ double s_sum[kWarps];
   __shared__ int s_twice, s_gap;
+  __shared__ uint32_t s_flags[kFlagWords][kThreads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int busy = min((A.K + 31) / 32, kWarps);  // warps with an entry
   List L;
@@ -126,11 +133,15 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
   L.s = L.log_p + A.K;
   float top = -INFINITY;
   int seen = 0, bad = 0;
+  float own[kEntries];  // logits on their way while the probabilities are worked out
   if (warp < busy) {
     const int32_t *ids = A.ids + row * A.ld_ids;
     const float *values = A.values + row * A.ld_values;
     const int n = A.n_list ? min(max(A.n_list[row], 0), A.K) : A.K;
-    for (int j = tid; j < A.K; j += kThreads) {
+#pragma unroll
+    for (int e = 0; e < kEntries; e++) {
+      const int j = tid + e * kThreads;
+      if (j >= A.K) break;
       int id = ids[j];
       float t = values[j];
       if (j >= n || id < 0 || id >= A.V) {
@@ -144,6 +155,7 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
       }
       L.id[j] = id;
       L.log_p[j] = t;
+      if (id >= 0 && id >= sp.c0 && id < sp.c1) own[e] = RowElem<T>::get(x_row + id);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
@@ -157,6 +169,8 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
   }
   for (int i = tid; i < A.bit_words / 4; i += kThreads) reinterpret_cast<uint4 *>(L.bits)[i] = make_uint4(0u, 0u, 0u, 0u);
   if (tid == 0) s_twice = s_gap = 0;
+#pragma unroll
+  for (int i = 0; i < kFlagWords; i++) s_flags[i][tid] = 0u;
   __syncthreads();
   top = -INFINITY;
   seen = bad = 0;
@@ -180,7 +194,10 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
   }
   if (warp < busy) {
     double sum = 0.0;
-    for (int j = tid; j < A.K; j += kThreads) {
+#pragma unroll
+    for (int e = 0; e < kEntries; e++) {
+      const int j = tid + e * kThreads;
+      if (j >= A.K) break;
       const int id = L.id[j];
       const float t = __fsub_rn(L.log_p[j], base);
       const float p = id >= 0 ? expf(t) : 0.0f;
@@ -189,7 +206,9 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
       sum += p;
       if (id >= 0 && id >= sp.c0 && id < sp.c1) {
         const uint32_t bit = 1u << ((id - sp.c0) & 31);
-        L.s[j] = RowElem<T>::get(x_row + id);
+        const int vec = (id - sp.c0) / RowElem<T>::N, batch = vec / kStep;
+        if (REST) atomicOr(&s_flags[batch >> 5][vec % kThreads], 1u << (batch & 31));
+        L.s[j] = own[e];
         if (atomicOr(&L.bits[(id - sp.c0) >> 5], bit) & bit) s_twice = 1;
       } else {
         L.id[j] = -1;
@@ -200,6 +219,8 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
     if (lane == 0) s_sum[warp] = sum;
   }
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kFlagWords; i++) L.flags[i] = s_flags[i][tid];
   double sum = 0.0;
   for (int i = 0; i < busy; i++) sum += s_sum[i];
   if (!REST) {
@@ -220,9 +241,9 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
   if (s_twice) {
     // the first entry of an id takes the probabilities of all, in list order
     __syncthreads();
-    float joined[PZ_TOP_K_MAX / kThreads];
+    float joined[kEntries];
 #pragma unroll
-    for (int e = 0; e < PZ_TOP_K_MAX / kThreads; e++) {
+    for (int e = 0; e < kEntries; e++) {
       const int j = tid + e * kThreads;
       joined[e] = -1.0f;
       if (j < A.K && L.id[j] >= 0) {
@@ -238,7 +259,7 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
     }
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < PZ_TOP_K_MAX / kThreads; e++) {
+    for (int e = 0; e < kEntries; e++) {
       const int j = tid + e * kThreads;
       if (j < A.K) {
         if (joined[e] == -1.0f) L.id[j] = -1;
@@ -250,8 +271,9 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
   return L;
 }
 
-// The row's columns as this thread sees them: vectors k0 + tid, k0 + tid +
-// kThreads, ... of the span.
+// The row's columns as a thread sees them: batches of kBatch vectors, kThreads
+// apart, from vector `kb + tid` on.  Batches that lie whole in the span and in
+// the row (the block's, all alike) take a path without a test per vector.
 template <typename T>
 struct Columns {
   static constexpr int N = RowElem<T>::N;
@@ -261,18 +283,54 @@ struct Columns {
   Span<T> sp;
   __device__ __forceinline__ Columns(const T *x_row, int V_, int part, int span)
       : row(x_row), V(V_), shift(row_shift(x_row)), whole(whole_vecs<T>(shift, V_)), sp(part, span, V_, shift) {}
-  __device__ __forceinline__ bool in_one_piece(int k) const { return k >= whole.first && k < whole.last; }
-  __device__ __forceinline__ uint4 load(int k) const {
-    return in_one_piece(k) ? load16(row + (k * N - shift)) : load_edge(row, V, k * N - shift);
+  __device__ __forceinline__ bool whole_batch(int kb) const {
+    return kb >= whole.first && kb + kStep <= min(sp.k1, whole.last);
   }
-  // Vector k into shared memory, asynchronously where it lies whole in the row.
-  __device__ __forceinline__ void fetch(uint4 *to, int k) const {
-    if (in_one_piece(k))
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
-                   "l"(row + (k * N - shift))
-                   : "memory");
-    else
-      *to = load_edge(row, V, k * N - shift);
+  __device__ __forceinline__ bool whole_vec(int k) const { return k >= whole.first && k < whole.last; }
+  __device__ __forceinline__ const T *at(int k) const { return row + (k * N - shift); }
+  // A batch into registers, -inf where there is no vector.
+  __device__ __forceinline__ void load(int kb, uint4 *raw) const {
+    const int k = kb + static_cast<int>(threadIdx.x);
+    if (whole_batch(kb)) {
+      const T *p = at(k);
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) raw[i] = load16(p + i * kThreads * N);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) {
+        const int v = k + i * kThreads;
+        raw[i] = make_uint4(RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2);
+        if (v < sp.k1) raw[i] = whole_vec(v) ? load16(at(v)) : load_edge(row, V, v * N - shift);
+      }
+    }
+  }
+  // The vectors [sp.k0, k_end) into shared memory, asynchronously where they
+  // lie whole in the row; every thread fetches those it reads itself.
+  __device__ __forceinline__ void fetch(uint4 *to, int k_end) const {
+    for (int k = sp.k0 + static_cast<int>(threadIdx.x); k < k_end; k += kThreads) {
+      uint4 *slot = to + (k - sp.k0);
+      if (whole_vec(k))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         static_cast<uint32_t>(__cvta_generic_to_shared(slot))),
+                     "l"(at(k))
+                     : "memory");
+      else
+        *slot = load_edge(row, V, k * N - shift);
+    }
+  }
+  __device__ __forceinline__ void held(const uint4 *from, int kb, int k_end, uint4 *raw) const {
+    const int k = kb + static_cast<int>(threadIdx.x);
+    const uint4 *p = from + (k - sp.k0);
+    if (kb + kStep <= k_end) {
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) raw[i] = p[i * kThreads];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) {
+        raw[i] = make_uint4(RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2);
+        if (k + i * kThreads < k_end) raw[i] = p[i * kThreads];
+      }
+    }
   }
 };
 
@@ -285,18 +343,28 @@ struct Gradient {
   __device__ __forceinline__ Gradient(T *g_row, int shift)
       : row(g_row),
         aligned(((reinterpret_cast<uintptr_t>(g_row) - static_cast<uintptr_t>(shift) * sizeof(T)) & 15u) == 0) {}
-  __device__ __forceinline__ void store(const Columns<T> &C, int k, const float *x) const {
-    const int c = k * N - C.shift;
-    if (aligned && C.in_one_piece(k))
-      store16(row + c, RowElem<T>::pack(x));
-    else
-      store_edge<N>(row, C.V, c, x);
+  __device__ __forceinline__ void store(const Columns<T> &C, int kb, int k_end, const uint4 *v) const {
+    const int k = kb + static_cast<int>(threadIdx.x);
+    if (aligned && C.whole_batch(kb)) {
+      T *p = row + (k * N - C.shift);
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) store16(p + i * kThreads * N, v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) {
+        const int at = k + i * kThreads;
+        if (at < k_end) {
+          if (aligned && C.whole_vec(at))
+            store16(row + (at * N - C.shift), v[i]);
+          else
+            store_edge(row, C.V, at * N - C.shift, v[i]);
+        }
+      }
+    }
   }
   __device__ __forceinline__ void zero(const Columns<T> &C) const {
-    float x[N];
-#pragma unroll
-    for (int j = 0; j < N; j++) x[j] = 0.0f;
-    for (int k = C.sp.k0 + threadIdx.x; k < C.sp.k1; k += kThreads) store(C, k, x);
+    const uint4 v[kBatch] = {};
+    for (int kb = C.sp.k0; kb < C.sp.k1; kb += kStep) store(C, kb, C.sp.k1, v);
   }
 };
 
@@ -395,79 +463,91 @@ __device__ __forceinline__ void grad_list(const DistillArgs &A, const List &L, c
   }
 }
 
+// One batch of the pass along the row: e times f.
 template <typename T>
-__device__ __forceinline__ void grad_vec(const uint4 &raw, float m, float c, float f, float *x) {
-  RowElem<T>::unpack(raw, x);
+__device__ __forceinline__ void grad_batch(uint4 *raw, float m, float c, float f) {
+  constexpr int P = RowElem<T>::N / 2;
+  const f32x2 m2 = pair(-m, -m), c2 = pair(c, c), f2 = pair(f, f);
 #pragma unroll
-  for (int j = 0; j < RowElem<T>::N; j++) x[j] = __fmul_rn(exp_from(x[j], m, c), f);
+  for (int i = 0; i < kBatch; i++) {
+    f32x2 x[P];
+    RowElem<T>::pairs(raw[i], x);
+#pragma unroll
+    for (int j = 0; j < P; j++) {
+      float a, b;
+      unpair(mul2(add2(x[j], m2), c2), a, b);
+      x[j] = mul2(pair(exp2_approx(a), exp2_approx(b)), f2);
+    }
+    raw[i] = RowElem<T>::pack_pairs(x);
+  }
 }
 
-// The vectors from `k` on, straight from global memory, the next batch in
-// flight while one is worked on.
+// The batches from kb on, straight from global memory, the next one in flight
+// while one is worked on (`now` holds the first).
 template <typename T>
 __device__ __forceinline__ void grad_stream(const Columns<T> &C, const Gradient<T> &G, const GradFactors &g, float c,
-                                            int k) {
-  uint4 now[kBatch], next[kBatch];
-#pragma unroll
-  for (int i = 0; i < kBatch; i++)
-    if (k + i * kThreads < C.sp.k1) now[i] = C.load(k + i * kThreads);
-  while (k < C.sp.k1) {
-    const int ahead = k + kBatch * kThreads;
-#pragma unroll
-    for (int i = 0; i < kBatch; i++)
-      if (ahead + i * kThreads < C.sp.k1) next[i] = C.load(ahead + i * kThreads);
-#pragma unroll
-    for (int i = 0; i < kBatch; i++) {
-      if (k + i * kThreads < C.sp.k1) {
-        float x[RowElem<T>::N];
-        grad_vec<T>(now[i], g.M_off, c, g.f, x);
-        G.store(C, k + i * kThreads, x);
-      }
-      now[i] = next[i];
+                                            int kb, uint4 *now) {
+  uint4 next[kBatch];
+  for (; kb < C.sp.k1; kb += 2 * kStep) {
+    if (kb + kStep < C.sp.k1) C.load(kb + kStep, next);
+    grad_batch<T>(now, g.M_off, c, g.f);
+    G.store(C, kb, C.sp.k1, now);
+    if (kb + kStep < C.sp.k1) {
+      if (kb + 2 * kStep < C.sp.k1) C.load(kb + 2 * kStep, now);
+      grad_batch<T>(next, g.M_off, c, g.f);
+      G.store(C, kb + kStep, C.sp.k1, next);
     }
-    k = ahead;
   }
 }
 
-// One batch into a thread's running maximum and sum.  REST: listed ids are
-// left out.
+// One batch into a thread's running maximum and sum (two sums, of the even
+// and the odd columns).  REST: listed ids are left out; few batches hold any.
 template <typename T, bool REST>
-__device__ __forceinline__ void sum_batch(const List &L, const Columns<T> &C, float c, uint4 *raw, int k, MaxSum &a) {
+__device__ __forceinline__ void sum_batch(const List &L, const Columns<T> &C, float c, uint4 *raw, int kb, float &m,
+                                          f32x2 &s) {
   constexpr int N = RowElem<T>::N;
-  float x[N];
-  float top = a.m;
+  if (REST) {
+    const int batch = (kb - C.sp.k0) / kStep;
+    const uint32_t f = batch < 32 ? L.flags[0] : L.flags[1];
+    if ((f >> (batch & 31)) & 1u) {
 #pragma unroll
-  for (int i = 0; i < kBatch; i++) {
-    const int at = k + i * kThreads;
-    if (at >= C.sp.k1) {
-      raw[i] = make_uint4(RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2, RowElem<T>::kNegInf2);
-    } else if (REST) {
-      const int u = (at - C.sp.k0) * N;
-      const uint32_t on = (L.bits[u >> 5] >> (u & 31)) & ((1u << N) - 1u);
-      if (on != 0u) {
-        RowElem<T>::unpack(raw[i], x);
+      for (int i = 0; i < kBatch; i++) {
+        const int u = (kb + static_cast<int>(threadIdx.x) + i * kThreads - C.sp.k0) * N;
+        const uint32_t on = u < C.sp.c1 - C.sp.c0 ? (L.bits[u >> 5] >> (u & 31)) & ((1u << N) - 1u) : 0u;
+        if (on != 0u) {
+          float x[N];
+          RowElem<T>::unpack(raw[i], x);
 #pragma unroll
-        for (int j = 0; j < N; j++)
-          if ((on >> j) & 1u) x[j] = -INFINITY;
-        raw[i] = RowElem<T>::pack(x);
+          for (int j = 0; j < N; j++)
+            if ((on >> j) & 1u) x[j] = -INFINITY;
+          raw[i] = RowElem<T>::pack(x);
+        }
       }
     }
-    top = fmaxf(top, RowElem<T>::max(raw[i]));
   }
+  float top = m;
+#pragma unroll
+  for (int i = 0; i < kBatch; i++) top = fmaxf(top, RowElem<T>::max(raw[i]));
   const float base = top > -INFINITY ? top : 0.0f;
-  float s = __fmul_rn(a.s, exp_from(a.m, base, c));
+  const f32x2 m2 = pair(-base, -base), c2 = pair(c, c);
+  const float scale = exp_from(m, base, c);
+  s = mul2(s, pair(scale, scale));
+  m = top;
 #pragma unroll
   for (int i = 0; i < kBatch; i++) {
-    RowElem<T>::unpack(raw[i], x);
+    f32x2 x[N / 2];
+    RowElem<T>::pairs(raw[i], x);
 #pragma unroll
-    for (int j = 0; j < N; j++) s = __fadd_rn(s, exp_from(x[j], base, c));
+    for (int j = 0; j < N / 2; j++) {
+      float a, b;
+      unpair(mul2(add2(x[j], m2), c2), a, b);
+      s = add2(s, pair(exp2_approx(a), exp2_approx(b)));
+    }
   }
-  a = MaxSum{top, s};
 }
 
 template <typename T, bool REST, bool GRAD>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const DistillArgs A) {
-  constexpr int STEP = kBatch * kThreads;
   __shared__ __align__(16) RowPart s_part[kMaxCluster];
   __shared__ MaxSum s_warp[kWarps][2];
   __shared__ double s_list[kWarps][2];
@@ -482,12 +562,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
 
   bool target = w != 0.0f;
   List L;
+  uint4 now[kBatch];
   uint4 *held = reinterpret_cast<uint4 *>(s_dyn);
   const int k_held = GRAD ? min(C.sp.k0 + A.resident, C.sp.k1) : C.sp.k0;  // the vectors before stay on chip
   if (target) {
-    if (GRAD) {
-      for (int k = C.sp.k0 + tid; k < k_held; k += kThreads) C.fetch(held + (k - C.sp.k0), k);
-    }
+    if (GRAD) C.fetch(held, k_held);
+    if (!GRAD) C.load(C.sp.k0, now);
     L = read_list<T, REST>(A, row, C.row, C.sp, s_dyn + static_cast<size_t>(A.resident) * 16);
     target = L.valid;
   }
@@ -505,34 +585,33 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
   cluster_arrive();
 
   // running maximum and sum of this thread's columns
-  MaxSum a{-INFINITY, 0.0f};
+  float m = -INFINITY;
+  f32x2 s = pair(0.0f, 0.0f);
   {
-    uint4 now[kBatch], next[kBatch];
-    int k = k_held + tid;
-#pragma unroll
-    for (int i = 0; i < kBatch; i++)
-      if (k + i * kThreads < C.sp.k1) now[i] = C.load(k + i * kThreads);
-    while (k < C.sp.k1) {
-#pragma unroll
-      for (int i = 0; i < kBatch; i++)
-        if (k + STEP + i * kThreads < C.sp.k1) next[i] = C.load(k + STEP + i * kThreads);
-      sum_batch<T, REST>(L, C, A.c, now, k, a);
-#pragma unroll
-      for (int i = 0; i < kBatch; i++) now[i] = next[i];
-      k += STEP;
+    uint4 next[kBatch];
+    int kb = k_held;
+    if (GRAD && kb < C.sp.k1) C.load(kb, now);
+    for (; kb < C.sp.k1; kb += 2 * kStep) {
+      if (kb + kStep < C.sp.k1) C.load(kb + kStep, next);
+      sum_batch<T, REST>(L, C, A.c, now, kb, m, s);
+      if (kb + kStep < C.sp.k1) {
+        if (kb + 2 * kStep < C.sp.k1) C.load(kb + 2 * kStep, now);
+        sum_batch<T, REST>(L, C, A.c, next, kb + kStep, m, s);
+      }
     }
   }
   if (GRAD) {
     asm volatile("cp.async.wait_all;" ::: "memory");  // a thread reads back what it fetched itself
-    Columns<T> H = C;
-    H.sp.k1 = k_held;
-    for (int k = C.sp.k0 + tid; k < k_held; k += STEP) {
-      uint4 now[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; i++)
-        if (k + i * kThreads < k_held) now[i] = held[k + i * kThreads - C.sp.k0];
-      sum_batch<T, REST>(L, H, A.c, now, k, a);
+    for (int kb = C.sp.k0; kb < k_held; kb += kStep) {
+      C.held(held, kb, k_held, now);
+      sum_batch<T, REST>(L, C, A.c, now, kb, m, s);
     }
+  }
+  MaxSum a{m, 0.0f};
+  {
+    float s0, s1;
+    unpair(s, s0, s1);
+    a.s = __fadd_rn(s0, s1);
   }
   a = join_lanes<32>(a, A.c);
   // and of its listed ids
@@ -551,13 +630,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
     r.row = join_lanes<kWarps>(s_warp[lane & (kWarps - 1)][0], A.c);
     r.list = MaxSum{-INFINITY, 0.0f};
     if (REST) r.list = join_lanes<kWarps>((lane & (kWarps - 1)) < busy ? s_warp[lane & (kWarps - 1)][1] : r.list, A.c);
-    const double ref = r.ref(), inv_T = 1.0 / static_cast<double>(A.T);
+    const double ref = r.ref();
     r.p = r.l = 0.0;
     for (int j = tid; j < A.K; j += kThreads) {
       const float p = L.p[j];
       if (L.id[j] < 0 || p == 0.0f) continue;
       r.p += p;
-      r.l += p * (L.log_p[j] - (L.s[j] - ref) * inv_T);
+      r.l += p * (L.log_p[j] - (L.s[j] - ref) * A.inv_T);
     }
     r.p = sum_lanes<32>(r.p);
     r.l = sum_lanes<32>(r.l);
@@ -594,32 +673,37 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
     if (!(R.M > -INFINITY)) R.M = 0.0f;
     if (!(R.M_off > -INFINITY)) R.M_off = R.M;
     if (GRAD && lane == 0) s_factors = grad_factors(L, R, A.c, by);
+    if (GRAD) asm volatile("bar.arrive 2, %0;" ::"r"(kThreads) : "memory");  // the others go on; the loss can wait
     if (part == 0) {
-      const double T_ = A.T;
       const double mass = sum_lanes<kMaxCluster>(mine.p);
-      double l = sum_lanes<kMaxCluster>(mine.l - mine.p * ((static_cast<double>(mine.ref()) - R.M) / T_));
+      double l = sum_lanes<kMaxCluster>(mine.l - mine.p * ((static_cast<double>(mine.ref()) - R.M) * A.inv_T));
       if (lane == 0) {
-        const double log_s = log(static_cast<double>(R.S));
+        const double T_ = A.T, log_s = log(static_cast<double>(R.S));
         l += mass * log_s;
         if (L.rho != 0.0f)
-          l += L.rho * (log(static_cast<double>(L.rho) / R.S_off) + log_s - (static_cast<double>(R.M_off) - R.M) / T_);
+          l += L.rho * (log(static_cast<double>(L.rho) / R.S_off) + log_s -
+                        (static_cast<double>(R.M_off) - R.M) * A.inv_T);
         if (R.S == 0.0f) l = INFINITY;  // every logit is -inf: the student has no distribution
         A.loss[row] = static_cast<float>(static_cast<double>(w) * T_ * T_ * l);
         if (A.stats) A.stats[row] = make_float4(R.M, R.S, R.M_off, R.S_off);
       }
     }
+    __syncwarp();
+  } else if (GRAD) {
+    asm volatile("bar.sync 2, %0;" ::"r"(kThreads) : "memory");
   }
   if constexpr (GRAD) {
-    __syncthreads();
     const GradFactors g = s_factors;
     const Gradient<T> G(static_cast<T *>(A.grad) + row * A.ld_grad, C.shift);
-#pragma unroll 2
-    for (int k = C.sp.k0 + tid; k < k_held; k += kThreads) {
-      float x[RowElem<T>::N];
-      grad_vec<T>(held[k - C.sp.k0], g.M_off, A.c, g.f, x);
-      G.store(C, k, x);
+    for (int kb = C.sp.k0; kb < k_held; kb += kStep) {
+      C.held(held, kb, k_held, now);
+      grad_batch<T>(now, g.M_off, A.c, g.f);
+      G.store(C, kb, k_held, now);
     }
-    if (k_held < C.sp.k1) grad_stream(C, G, g, A.c, k_held + tid);
+    if (k_held < C.sp.k1) {
+      C.load(k_held, now);
+      grad_stream(C, G, g, A.c, k_held, now);
+    }
     __syncthreads();
     grad_list(A, L, g, G.row, by);
   }
@@ -639,7 +723,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_backward_kernel(
   const float4 st = A.stats[row];
   bool target = w != 0.0f;
   List L;
+  uint4 now[kBatch];
   if (target) {
+    C.load(C.sp.k0, now);
     L = read_list<T, REST>(A, row, C.row, C.sp, s_dyn);
     target = L.valid;
   }
@@ -650,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_backward_kernel(
   const float by = __fmul_rn(__fmul_rn(w, A.T), up);
   const GradFactors g = grad_factors(L, RowSums{st.x, st.y, st.z, st.w}, A.c, by);
   // (read_list has read the listed logits: the gradient may lie over them)
-  grad_stream(C, G, g, A.c, C.sp.k0 + static_cast<int>(threadIdx.x));
+  grad_stream(C, G, g, A.c, C.sp.k0, now);
   __syncthreads();
   grad_list(A, L, g, G.row, by);
 }
@@ -684,6 +770,7 @@ cudaError_t launch_distill_as(DistillArgs &A, cudaStream_t st) {
   A.parts = parts;
   A.span = (vecs + parts - 1) / parts;
   A.resident = GRAD ? (A.span < kResident / 16 ? A.span : kResident / 16) : 0;
+  if (A.span > kMaxSpan) return cudaErrorInvalidConfiguration;
   const int64_t ctas = static_cast<int64_t>(A.N) * parts;
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
   const size_t smem = distill_smem<T>(A);
@@ -767,6 +854,7 @@ pz_status distill_args(const char *who, DistillArgs *A, const void *logits, pz_d
   A->weight = t->weight;
   A->T = t->temperature;
   A->c = static_cast<float>(1.4426950408889634 / static_cast<double>(t->temperature));
+  A->inv_T = 1.0 / static_cast<double>(t->temperature);
   A->rest = t->mode == PZ_DISTILL_REST ? 1 : 0;
   return PZ_OK;
 }

@@ -13,6 +13,28 @@
 
 namespace pz {
 
+// Two fp32 values in one 64-bit register: sm_100 adds and multiplies both in
+// one instruction, each rounded as on its own.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(f32x2 p, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 struct bf16_t {  // a bf16 element as it lies in memory
   uint16_t bits;
 };
@@ -33,6 +55,16 @@ struct RowElem<float> {
   }
   static __device__ __forceinline__ uint4 pack(const float *x) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+  static __device__ __forceinline__ void pairs(const uint4 &u, f32x2 *p) {
+    p[0] = pair(__uint_as_float(u.x), __uint_as_float(u.y));
+    p[1] = pair(__uint_as_float(u.z), __uint_as_float(u.w));
+  }
+  static __device__ __forceinline__ uint4 pack_pairs(const f32x2 *p) {
+    float x[4];
+    unpair(p[0], x[0], x[1]);
+    unpair(p[1], x[2], x[3]);
+    return pack(x);
   }
   static __device__ __forceinline__ float max(const uint4 &u) {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
@@ -64,6 +96,21 @@ struct RowElem<bf16_t> {
   }
   static __device__ __forceinline__ uint4 pack(const float *x) {
     return make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+  }
+  static __device__ __forceinline__ void pairs(const uint4 &u, f32x2 *p) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) p[j] = pair(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ uint4 pack_pairs(const f32x2 *p) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      float lo, hi;
+      unpair(p[j], lo, hi);
+      w[j] = pack2(lo, hi);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
   // the largest value that is not NaN (NaN where all are), two at a time
   static __device__ __forceinline__ float max(const uint4 &u) {
@@ -113,9 +160,13 @@ __device__ __noinline__ uint4 load_edge(const T *row, int V, int c) {
     x[j] = (c + j >= 0 && c + j < V) ? RowElem<T>::get(row + c + j) : __int_as_float(0xFF800000);
   return RowElem<T>::pack(x);
 }
-// Columns [c, c + N) of a row, those inside [0, V), one at a time.
-template <int N, typename T>
-__device__ __noinline__ void store_edge(T *row, int V, int c, const float *x) {
+// A packed vector to the columns [c, c + N) of a row, those inside [0, V).
+template <typename T>
+__device__ __noinline__ void store_edge(T *row, int V, int c, uint4 v) {
+  constexpr int N = RowElem<T>::N;
+  float x[N];
+  RowElem<T>::unpack(v, x);
+#pragma unroll
   for (int j = 0; j < N; j++)
     if (c + j >= 0 && c + j < V) RowElem<T>::put(row + c + j, x[j]);
 }
