@@ -41,15 +41,15 @@
 namespace pz {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;              // 16-byte vectors that a thread works on at a time
 constexpr int kStep = kBatch * kThreads;
 constexpr int kEntries = PZ_TOP_K_MAX / kThreads;  // most list entries of a thread
-constexpr int kFlagWords = 2;
+constexpr int kFlagWords = 4;
 constexpr int kMaxSpan = kFlagWords * 32 * kStep;   // vectors of a span: a flag per batch of a thread
 constexpr int kMaxCluster = 8;         // the portable cluster size
-constexpr int kCtasPerSm = 4;
+constexpr int kCtasPerSm = 7;
 constexpr int kResident = 64 * 1024;   // most bytes of a row that a CTA keeps in shared memory
 
 struct DistillArgs {
@@ -113,16 +113,31 @@ struct Span {
   }
 };
 
+// A thread's first entry of the row's list, on its way before anything is
+// known about the row.
+struct Entry {
+  int id, n;
+  float value;
+  __device__ __forceinline__ Entry(const DistillArgs &A, int64_t row) : id(-1), n(A.K), value(0.0f) {
+    const int j = threadIdx.x;
+    if (j < A.K) {
+      if (A.n_list) n = min(max(A.n_list[row], 0), A.K);
+      id = A.ids[row * A.ld_ids + j];
+      value = A.values[row * A.ld_values + j];
+    }
+  }
+};
+
 // Reads the row's list: the probabilities and, of the ids in the CTA's
 // columns, bits and logits.  Two barriers of the block, the second one last.
 template <typename T, bool REST>
-__device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, const T *x_row, const Span<T> &sp,
-                                          unsigned char *smem) {
+__device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, const Entry &first, const T *x_row,
+                                          const Span<T> &sp, unsigned char *smem) {
   __shared__ float s_top[kWarps];
   __shared__ int s_seen[kWarps], s_bad[kWarps];
   __shared__ double s_sum[kWarps];
   __shared__ int s_twice, s_gap;
-  __shared__ uint32_t s_flags[kFlagWords][kThreads];
+  __shared__ uint32_t s_flags[REST ? kFlagWords : 1][REST ? kThreads : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int busy = min((A.K + 31) / 32, kWarps);  // warps with an entry
   List L;
@@ -137,14 +152,13 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
   if (warp < busy) {
     const int32_t *ids = A.ids + row * A.ld_ids;
     const float *values = A.values + row * A.ld_values;
-    const int n = A.n_list ? min(max(A.n_list[row], 0), A.K) : A.K;
 #pragma unroll
     for (int e = 0; e < kEntries; e++) {
       const int j = tid + e * kThreads;
       if (j >= A.K) break;
-      int id = ids[j];
-      float t = values[j];
-      if (j >= n || id < 0 || id >= A.V) {
+      int id = e == 0 ? first.id : ids[j];
+      float t = e == 0 ? first.value : values[j];
+      if (j >= first.n || id < 0 || id >= A.V) {
         id = -1;
         t = -INFINITY;
       } else {
@@ -169,8 +183,10 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
   }
   for (int i = tid; i < A.bit_words / 4; i += kThreads) reinterpret_cast<uint4 *>(L.bits)[i] = make_uint4(0u, 0u, 0u, 0u);
   if (tid == 0) s_twice = s_gap = 0;
+  if (REST) {
 #pragma unroll
-  for (int i = 0; i < kFlagWords; i++) s_flags[i][tid] = 0u;
+    for (int i = 0; i < kFlagWords; i++) s_flags[i][tid] = 0u;
+  }
   __syncthreads();
   top = -INFINITY;
   seen = bad = 0;
@@ -206,9 +222,11 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
       sum += p;
       if (id >= 0 && id >= sp.c0 && id < sp.c1) {
         const uint32_t bit = 1u << ((id - sp.c0) & 31);
-        const int vec = (id - sp.c0) / RowElem<T>::N, batch = vec / kStep;
-        if (REST) atomicOr(&s_flags[batch >> 5][vec % kThreads], 1u << (batch & 31));
         L.s[j] = own[e];
+        if (REST) {
+          const int vec = (id - sp.c0) / RowElem<T>::N, batch = vec / kStep;
+          atomicOr(&s_flags[batch >> 5][vec % kThreads], 1u << (batch & 31));
+        }
         if (atomicOr(&L.bits[(id - sp.c0) >> 5], bit) & bit) s_twice = 1;
       } else {
         L.id[j] = -1;
@@ -219,8 +237,10 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
     if (lane == 0) s_sum[warp] = sum;
   }
   __syncthreads();
+  if (REST) {
 #pragma unroll
-  for (int i = 0; i < kFlagWords; i++) L.flags[i] = s_flags[i][tid];
+    for (int i = 0; i < kFlagWords; i++) L.flags[i] = s_flags[i][tid];
+  }
   double sum = 0.0;
   for (int i = 0; i < busy; i++) sum += s_sum[i];
   if (!REST) {
@@ -307,16 +327,27 @@ struct Columns {
   // The vectors [sp.k0, k_end) into shared memory, asynchronously where they
   // lie whole in the row; every thread fetches those it reads itself.
   __device__ __forceinline__ void fetch(uint4 *to, int k_end) const {
-    for (int k = sp.k0 + static_cast<int>(threadIdx.x); k < k_end; k += kThreads) {
+    for (int kb = sp.k0; kb < k_end; kb += kStep) {
+      const int k = kb + static_cast<int>(threadIdx.x);
       uint4 *slot = to + (k - sp.k0);
-      if (whole_vec(k))
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                         static_cast<uint32_t>(__cvta_generic_to_shared(slot))),
-                     "l"(at(k))
-                     : "memory");
-      else
-        *slot = load_edge(row, V, k * N - shift);
+      if (whole_batch(kb) && kb + kStep <= k_end) {
+        const T *p = at(k);
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) copy16(slot + i * kThreads, p + i * kThreads * N);
+      } else {
+        for (int v = k; v < min(kb + kStep, k_end); v += kThreads, slot += kThreads) {
+          if (whole_vec(v))
+            copy16(slot, at(v));
+          else
+            *slot = load_edge(row, V, v * N - shift);
+        }
+      }
     }
+  }
+  static __device__ __forceinline__ void copy16(uint4 *to, const T *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                 "l"(from)
+                 : "memory");
   }
   __device__ __forceinline__ void held(const uint4 *from, int kb, int k_end, uint4 *raw) const {
     const int k = kb + static_cast<int>(threadIdx.x);
@@ -414,7 +445,11 @@ struct RowPart {
 };
 
 // The row's cluster: all CTAs have to arrive before any passes the wait.
+// Threads that wrote nothing for the others arrive without a fence.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // Copies v to the same shared variable of CTA `rank` of the cluster.
@@ -508,7 +543,10 @@ __device__ __forceinline__ void sum_batch(const List &L, const Columns<T> &C, fl
   constexpr int N = RowElem<T>::N;
   if (REST) {
     const int batch = (kb - C.sp.k0) / kStep;
-    const uint32_t f = batch < 32 ? L.flags[0] : L.flags[1];
+    uint32_t f = L.flags[0];
+#pragma unroll
+    for (int i = 1; i < kFlagWords; i++)
+      if (batch >= 32 * i) f = L.flags[i];
     if ((f >> (batch & 31)) & 1u) {
 #pragma unroll
       for (int i = 0; i < kBatch; i++) {
@@ -563,12 +601,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
   bool target = w != 0.0f;
   List L;
   uint4 now[kBatch];
+  const Entry first(A, row);
   uint4 *held = reinterpret_cast<uint4 *>(s_dyn);
   const int k_held = GRAD ? min(C.sp.k0 + A.resident, C.sp.k1) : C.sp.k0;  // the vectors before stay on chip
   if (target) {
     if (GRAD) C.fetch(held, k_held);
     if (!GRAD) C.load(C.sp.k0, now);
-    L = read_list<T, REST>(A, row, C.row, C.sp, s_dyn + static_cast<size_t>(A.resident) * 16);
+    L = read_list<T, REST>(A, row, first, C.row, C.sp, s_dyn + static_cast<size_t>(A.resident) * 16);
     target = L.valid;
   }
   if (!target) {  // the whole cluster leaves
@@ -582,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
     }
     return;
   }
-  cluster_arrive();
+  cluster_arrive_relaxed();
 
   // running maximum and sum of this thread's columns
   float m = -INFINITY;
@@ -655,10 +694,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
     if (warp == 0) {
       cluster_wait();  // every CTA of the row runs: its shared memory may be written
       if (lane < A.parts) put_remote(&s_part[part], r, lane);
+      cluster_arrive();
     }
   }
-  if (warp != 0) cluster_wait();
-  cluster_arrive();
+  if (warp != 0) {
+    cluster_wait();
+    cluster_arrive_relaxed();
+  }
   cluster_wait();
   if (warp == 0) {
     const RowPart none{{-INFINITY, 0.0f}, {-INFINITY, 0.0f}, 0.0, 0.0};
@@ -724,9 +766,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_backward_kernel(
   bool target = w != 0.0f;
   List L;
   uint4 now[kBatch];
+  const Entry first(A, row);
   if (target) {
     C.load(C.sp.k0, now);
-    L = read_list<T, REST>(A, row, C.row, C.sp, s_dyn);
+    L = read_list<T, REST>(A, row, first, C.row, C.sp, s_dyn);
     target = L.valid;
   }
   if (!target) {
