@@ -69,6 +69,11 @@ struct RowElem<float> {
   static __device__ __forceinline__ float max(const uint4 &u) {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
   }
+  // the elements whose bit is set, -inf for the others
+  static __device__ __forceinline__ uint4 keep(const uint4 &u, uint32_t bits) {
+    return make_uint4((bits & 1u) ? u.x : kNegInf2, (bits & 2u) ? u.y : kNegInf2, (bits & 4u) ? u.z : kNegInf2,
+                      (bits & 8u) ? u.w : kNegInf2);
+  }
   static constexpr uint32_t kNegInf2 = 0xFF800000u;  // what a 32-bit word of -inf holds
 };
 
@@ -118,6 +123,17 @@ struct RowElem<bf16_t> {
     const __nv_bfloat162 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
     return fmaxf(__low2float(m), __high2float(m));
   }
+  // Selectors of a byte permutation for four elements: 0x54 and 0x76 take the
+  // two bytes of an element from the second operand, 0x10 and 0x32 (0x44
+  // less) from the first.  The product spreads four bits over four bytes.
+  static __device__ __forceinline__ uint32_t selectors(uint32_t bits) {
+    return 0x76547654u - (((bits & 0xFu) * 0x00204081u) & 0x01010101u) * 0x44u;
+  }
+  static __device__ __forceinline__ uint4 keep(const uint4 &u, uint32_t bits) {
+    const uint32_t lo = selectors(bits), hi = selectors(bits >> 4);
+    return make_uint4(__byte_perm(u.x, kNegInf2, lo), __byte_perm(u.y, kNegInf2, lo >> 16),
+                      __byte_perm(u.z, kNegInf2, hi), __byte_perm(u.w, kNegInf2, hi >> 16));
+  }
   static constexpr uint32_t kNegInf2 = 0xFF80FF80u;
 };
 
@@ -139,6 +155,8 @@ __device__ __forceinline__ uint4 load16(const void *p) {
 __device__ __forceinline__ void store16(void *p, const uint4 &v) {
   __stcs(reinterpret_cast<uint4 *>(p), v);
 }
+// A store of what is written again soon: it stays in L2.
+__device__ __forceinline__ void store16_keep(void *p, const uint4 &v) { *reinterpret_cast<uint4 *>(p) = v; }
 
 // Vectors [first, last) of a row lie in it whole.
 struct WholeVecs {

@@ -16,15 +16,16 @@
 // Bound: HBM.  Out of place every logit is read and written once; in place
 // only the vectors that something changes are touched.
 //
-// One CTA takes a tile of a row's columns.  It first has its logits on their
-// way to registers, then reads the whole of the row's history and bias list
-// (a few KB, from L2 after the row's first tile) and keeps what falls into
-// its columns: a count per column and the index of the last bias entry per
-// column, in shared memory, with one bit per column that says whether either
-// is there.  Counts per column need no bound on the history's length and no
-// hashing, and integer atomics give the same sums in any order.  Every
-// vector is then changed by the thread that read it and written once: no
-// column has two writers, so the output may be the input.
+// A CTA takes a part of a row.  Four warps pass along its columns and know
+// the mask alone.  Two more work out the listed ids meanwhile: those that lie
+// in the CTA's columns go into a hash table in shared memory, which counts how
+// often each occurs in the history and remembers its last bias entry (integer
+// atomics: the same sums in any order); their new values, computed from the
+// input, are stored over what the pass wrote once it is through.  In place
+// the pass changes no allowed id, so both ways a value is read before
+// anything lies over it.  A part with more distinct ids than the table takes
+// is done in classes of the ids' hash, each as small as it needs: histories
+// may have any length.
 #include "pz_device.cuh"
 #include "pz_rowvec.cuh"
 #include "pz_status.cuh"
@@ -32,14 +33,15 @@
 namespace pz {
 namespace {
 
-constexpr int kRulesThreads = 256;
+constexpr int kRulesThreads = 128;
 
 struct RulesArgs {
   const void *in;
   void *out;
   int64_t ld_in, ld_out;
   int V;
-  int tiles;  // column tiles per row; one more CTA per row counts the mask when n_allowed is given
+  int parts;  // CTAs per row; one more counts the mask when n_allowed is given
+  int span;   // vectors per CTA
   const pz_sampler_config *cfg;
   const int32_t *hist, *hist_off;
   const int32_t *bias_ids;
@@ -62,172 +64,360 @@ __device__ __forceinline__ const uint32_t *mask_row(const RulesArgs &A, int row)
 
 // Allowed ids of a row: the set bits of its mask among the columns [0, V).
 __device__ void count_allowed(const RulesArgs &A, int row) {
-  __shared__ int s_part[kRulesThreads / 32];
+  __shared__ int s_sum;
   const uint32_t *m = mask_row(A, row);
-  int n = 0;
-  if (m != nullptr) {
-    const int words = (A.V + 31) / 32;
-    for (int i = threadIdx.x; i < words; i += kRulesThreads) {
-      uint32_t w = m[i];
-      if (i == words - 1 && (A.V & 31) != 0) w &= (1u << (A.V & 31)) - 1u;
-      n += __popc(w);
-    }
-    n = __reduce_add_sync(0xFFFFFFFFu, n);
-    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = n;
-    __syncthreads();
-    n = 0;
-    for (int w = 0; w < kRulesThreads / 32; w++) n += s_part[w];
-  } else {
-    n = A.V;
+  if (m == nullptr) {
+    if (threadIdx.x == 0) A.n_allowed[row] = A.V;
+    return;
   }
-  if (threadIdx.x == 0) A.n_allowed[row] = n;
+  if (threadIdx.x == 0) s_sum = 0;
+  __syncthreads();
+  int n = 0;
+  const int words = (A.V + 31) / 32;
+  for (int i = threadIdx.x; i < words; i += blockDim.x) {
+    uint32_t w = m[i];
+    if (i == words - 1 && (A.V & 31) != 0) w &= (1u << (A.V & 31)) - 1u;
+    n += __popc(w);
+  }
+  n = __reduce_add_sync(0xFFFFFFFFu, n);
+  if ((threadIdx.x & 31) == 0) atomicAdd(&s_sum, n);
+  __syncthreads();
+  if (threadIdx.x == 0) A.n_allowed[row] = s_sum;
 }
 
-// VPT vectors of 16 input bytes per thread.  The tile's columns are counted
-// from c0, which lies up to one vector before column 0 in the first tile.
-template <typename Ti, typename To, int VPT, bool INPLACE, bool LISTS>
-__global__ void __launch_bounds__(kRulesThreads) rules_kernel(const RulesArgs A) {
+constexpr int kSlots = 1024;     // of the hash table
+constexpr int kProbes = 32;      // a longer run of taken slots counts as a full table
+constexpr int kRulesBatch = 4;   // vectors that a thread has in flight
+constexpr int kRulesStep = kRulesBatch * kRulesThreads;
+
+constexpr int kListThreads = 64;  // beside the pass's, in a CTA with lists
+
+struct Table {
+  int32_t key[kSlots];    // id or -1
+  int32_t count[kSlots];  // occurrences in the history
+  int32_t last[kSlots];   // last bias entry + 1
+  uint16_t slot[kSlots];  // the taken slots, in the order they were taken
+  float value[kSlots];    // by that order: the new value
+  int taken;
+  int full;
+};
+
+// The lists of a row in the columns [c0, c1).
+template <typename Ti, typename To>
+struct Lists {
+  const int32_t *hist, *bias_ids;  // of this row
+  const float *bias_vals;
+  int n_hist, n_bias;
+  int c0, c1;
+  RowPlan P;
+  uint32_t cls = 0;  // the class of ids that is being worked on: those whose hash ends in these bits
+  int bits = 0;
+
+  __device__ __forceinline__ Lists(const RulesArgs &A, int row, int c0_, int c1_)
+      : hist(nullptr), bias_ids(nullptr), bias_vals(nullptr), n_hist(0), n_bias(0), c0(c0_), c1(c1_), P{} {
+    if (A.hist != nullptr) {
+      const int from = A.hist_off[row], to = A.hist_off[row + 1];
+      P = plan_row(A.cfg[row], A.V);
+      hist = A.hist + from;
+      n_hist = P.pen_on ? to - from : 0;
+    }
+    if (A.bias_ids != nullptr) {
+      const int from = A.bias_off[row];
+      bias_ids = A.bias_ids + from;
+      bias_vals = A.bias_vals + from;
+      n_bias = A.bias_off[row + 1] - from;
+    }
+  }
+  static __device__ __forceinline__ uint32_t hash(int id) {  // odd factor: one to one
+    return static_cast<uint32_t>(id) * 0x9E3779B1u;
+  }
+  // The threads that work on the lists, and their barrier.
+  static __device__ __forceinline__ int self() { return static_cast<int>(threadIdx.x) - kRulesThreads; }
+  static __device__ __forceinline__ void sync() { asm volatile("bar.sync 1, %0;" ::"r"(kListThreads) : "memory"); }
+  // One list's ids of the class into the table.
+  template <bool BIAS>
+  __device__ __forceinline__ void fill(Table &S, const int32_t *ids, int n) const {
+    constexpr int G = 8;  // ids in flight
+    const uint32_t low = bits >= 32 ? 0xFFFFFFFFu : (1u << bits) - 1u;
+    for (int64_t j0 = self(); j0 < n; j0 += G * kListThreads) {
+      int id[G];
+#pragma unroll
+      for (int g = 0; g < G; g++) id[g] = j0 + g * kListThreads < n ? ids[j0 + g * kListThreads] : -1;
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const int t = id[g];
+        if (t < c0 || t >= c1 || (hash(t) & low) != cls) continue;  // (c0 >= 0)
+        uint32_t at = hash(t) >> 22;
+        static_assert(kSlots == 1 << 10, "the slot is the hash's top 10 bits");
+        int tries = 0;
+        for (; tries < kProbes; tries++, at = (at + 1) % kSlots) {
+          const int was = atomicCAS(&S.key[at], -1, t);
+          if (was == -1) S.slot[atomicAdd(&S.taken, 1)] = static_cast<uint16_t>(at);
+          if (was == -1 || was == t) break;
+        }
+        if (tries == kProbes)
+          S.full = 1;
+        else if (BIAS)
+          atomicMax(&S.last[at], static_cast<int>(j0) + g * kListThreads + 1);
+        else
+          atomicAdd(&S.count[at], 1);
+      }
+    }
+  }
+  // The next class that fits the table, from the present one on.
+  __device__ __forceinline__ void build(Table &S) {
+    for (;;) {
+      for (int i = self(); i < kSlots / 4; i += kListThreads) {
+        reinterpret_cast<int4 *>(S.key)[i] = make_int4(-1, -1, -1, -1);
+        reinterpret_cast<int4 *>(S.count)[i] = make_int4(0, 0, 0, 0);
+        reinterpret_cast<int4 *>(S.last)[i] = make_int4(0, 0, 0, 0);
+      }
+      if (self() == 0) S.taken = S.full = 0;
+      sync();
+      fill<false>(S, hist, n_hist);
+      fill<true>(S, bias_ids, n_bias);
+      sync();
+      if (!S.full) return;
+      bits++;  // half of the class (32 bits leave one id)
+      sync();
+    }
+  }
+  // To the next class; false when there is none.
+  __device__ __forceinline__ bool advance() {
+    while (bits > 0 && ((cls >> (bits - 1)) & 1u)) {
+      bits--;
+      cls &= (1u << bits) - 1u;
+    }
+    if (bits == 0) return false;
+    cls |= 1u << (bits - 1);
+    return true;
+  }
+  // The new values of the taken slots (a slot whose id the mask takes: none).
+  __device__ __forceinline__ void gather(Table &S, const Ti *in, const uint32_t *m) const {
+    constexpr int G = 4;  // loads in flight
+    const int n = S.taken;
+    for (int i0 = self(); i0 < n; i0 += G * kListThreads) {
+      float x[G];
+      bool on[G];
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        on[g] = false;
+        if (i0 + g * kListThreads < n) {
+          const int t = S.key[S.slot[i0 + g * kListThreads]];
+          x[g] = RowElem<Ti>::get(in + t);
+          on[g] = m == nullptr || ((m[t >> 5] >> (t & 31)) & 1u);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        if (i0 + g * kListThreads >= n) continue;
+        const int at = S.slot[i0 + g * kListThreads];
+        float y = x[g];
+        if (S.count[at] > 0) y = penalize(y, S.count[at], P);
+        if (S.last[at] > 0) y = __fadd_rn(y, bias_vals[S.last[at] - 1]);
+        S.value[i0 + g * kListThreads] = y;
+        if (!on[g]) S.key[at] = -1;
+      }
+    }
+  }
+  __device__ __forceinline__ void scatter(const Table &S, To *out) const {
+    for (int i = self(); i < S.taken; i += kListThreads) {
+      const int t = S.key[S.slot[i]];
+      if (t >= 0) RowElem<To>::put(out + t, S.value[i]);
+    }
+  }
+};
+
+// The pass along the columns of the vectors [k0, k1): the mask alone.  A
+// thread's vectors are kRulesThreads apart, a multiple of 32 columns, so
+// their bits lie at one offset of words a fixed step apart.
+template <typename Ti, typename To, bool INPLACE, bool KEEP>
+struct MaskPass {
+  static constexpr int N = RowElem<Ti>::N;
+  static constexpr uint32_t ALL = (1u << N) - 1u;
+  static constexpr int WORDS = kRulesThreads * N / 32;  // between a thread's vectors
+  static_assert(kRulesThreads * N % 32 == 0, "a thread's vectors share their bit offset");
+  const Ti *in;
+  To *out;
+  const uint32_t *m;
+  int V, shift, words, k1;
+  WholeVecs whole;
+  bool aligned;
+
+  __device__ __forceinline__ bool whole_batch(int kb) const {  // the block's batch from vector kb on
+    return kb >= whole.first && kb + kRulesStep <= min(k1, whole.last);
+  }
+  // The mask bits of the columns [c, c + N).  c may lie up to a vector before
+  // column 0; bits outside the words are 0.
+  __device__ __forceinline__ uint32_t bits_at(int c) const {
+    const int at = c >> 5, off = c & 31;
+    uint32_t w = at >= 0 ? __ldg(m + at) >> off : 0u;
+    if (off > 32 - N && at + 1 < words) w |= __ldg(m + at + 1) << (32 - off);
+    return w & ALL;
+  }
+  __device__ __forceinline__ void load(int kb, uint4 *raw, uint32_t *allow) const {
+    const int k = kb + static_cast<int>(threadIdx.x);
+    if (whole_batch(kb)) {
+      const int c = k * N - shift;
+      if (!INPLACE) {
+#pragma unroll
+        for (int i = 0; i < kRulesBatch; i++) raw[i] = load16(in + c + i * kRulesThreads * N);
+      }
+      if (m == nullptr) return;
+      const int off = c & 31;
+      const uint32_t *p = m + (c >> 5);
+      if (shift == 0) {  // off + N <= 32
+#pragma unroll
+        for (int i = 0; i < kRulesBatch; i++) allow[i] = (__ldg(p + i * WORDS) >> off) & ALL;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRulesBatch; i++) allow[i] = bits_at(c + i * kRulesThreads * N);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRulesBatch; i++) {
+        const int v = k + i * kRulesThreads;
+        allow[i] = ALL;
+        if (v < k1) {
+          if (!INPLACE) raw[i] = vec(v);
+          if (m != nullptr) allow[i] = bits_at(v * N - shift);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ uint4 vec(int k) const {
+    return k >= whole.first && k < whole.last ? load16(in + (k * N - shift)) : load_edge(in, V, k * N - shift);
+  }
+  __device__ __forceinline__ void store(int kb, uint4 *raw, const uint32_t *allow) const {
+    const int k = kb + static_cast<int>(threadIdx.x);
+    if (INPLACE) {  // only the vectors that keep some of their values are read
+#pragma unroll
+      for (int i = 0; i < kRulesBatch; i++)
+        if (allow[i] != ALL && allow[i] != 0u) raw[i] = vec(k + i * kRulesThreads);
+    }
+    if (m != nullptr) {
+#pragma unroll
+      for (int i = 0; i < kRulesBatch; i++) raw[i] = RowElem<Ti>::keep(raw[i], allow[i]);
+    }
+    if (whole_batch(kb) && aligned) {
+      To *p = out + (k * N - shift);
+#pragma unroll
+      for (int i = 0; i < kRulesBatch; i++)
+        if (!INPLACE || allow[i] != ALL) put(p + i * kRulesThreads * N, raw[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRulesBatch; i++) {
+        const int v = k + i * kRulesThreads;
+        if (v >= k1 || (INPLACE && allow[i] == ALL)) continue;
+        if (aligned && v >= whole.first && v < whole.last)
+          put(out + (v * N - shift), raw[i]);
+        else
+          put_edge(v * N - shift, raw[i]);
+      }
+    }
+  }
+  // KEEP: listed ids are stored over some of it.
+  static __device__ __forceinline__ void put16(To *p, const uint4 &v) { KEEP ? store16_keep(p, v) : store16(p, v); }
+  static __device__ __forceinline__ void put(To *p, const uint4 &v) {
+    if constexpr (sizeof(Ti) == sizeof(To)) {
+      put16(p, v);
+    } else {
+      float x[N];
+      RowElem<Ti>::unpack(v, x);
+#pragma unroll
+      for (int j = 0; j < N; j += RowElem<To>::N) put16(p + j, RowElem<To>::pack(x + j));
+    }
+  }
+  __device__ __forceinline__ void put_edge(int c, const uint4 &v) const {
+    if constexpr (sizeof(Ti) == sizeof(To)) {
+      store_edge(out, V, c, v);
+    } else {
+      float x[N];
+      RowElem<Ti>::unpack(v, x);
+#pragma unroll
+      for (int j = 0; j < N; j += RowElem<To>::N) store_edge(out, V, c + j, RowElem<To>::pack(x + j));
+    }
+  }
+  // The next batch is in flight while one is worked on.
+  __device__ __forceinline__ void run(int k0) const {
+    if (INPLACE && m == nullptr) return;
+    uint4 a[kRulesBatch], b[kRulesBatch];
+    uint32_t aa[kRulesBatch], ab[kRulesBatch];
+    load(k0, a, aa);
+    for (int kb = k0; kb < k1; kb += 2 * kRulesStep) {
+      if (kb + kRulesStep < k1) load(kb + kRulesStep, b, ab);
+      store(kb, a, aa);
+      if (kb + kRulesStep < k1) {
+        if (kb + 2 * kRulesStep < k1) load(kb + 2 * kRulesStep, a, aa);
+        store(kb + kRulesStep, b, ab);
+      }
+    }
+  }
+};
+
+// kRulesThreads threads for the pass; with lists, kListThreads more.
+template <typename Ti, typename To, bool INPLACE, bool LISTS>
+__global__ void __launch_bounds__(kRulesThreads + (LISTS ? kListThreads : 0), LISTS ? 5 : 7)
+    rules_kernel(const RulesArgs A) {
   constexpr int N = RowElem<Ti>::N;
-  constexpr int TILE = kRulesThreads * VPT * N;
-  constexpr int WORDS = TILE / 32;
-  __shared__ uint32_t s_allow[WORDS];
-  __shared__ uint32_t s_touch[LISTS ? WORDS : 1];
-  extern __shared__ __align__(16) int32_t s_dyn[];  // counts [TILE], last bias entries [TILE]
-  const int per_row = A.tiles + (A.n_allowed != nullptr ? 1 : 0);
+  const int per_row = A.parts + (A.n_allowed != nullptr ? 1 : 0);
   const int row = blockIdx.x / per_row;
-  const int tile = blockIdx.x - row * per_row;
-  const int tid = threadIdx.x;
-  if (tile == A.tiles) {
+  const int part = blockIdx.x - row * per_row;
+  if (part == A.parts) {
     count_allowed(A, row);
     return;
   }
   const Ti *in = static_cast<const Ti *>(A.in) + static_cast<int64_t>(row) * A.ld_in;
   To *out = static_cast<To *>(A.out) + static_cast<int64_t>(row) * A.ld_out;
   const int shift = row_shift(in);
-  const int c0 = tile * TILE - shift;
-  if (c0 >= A.V) return;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(out) - static_cast<uintptr_t>(shift) * sizeof(To)) & 15u) == 0;
-  const int k0 = tile * (kRulesThreads * VPT) + tid;
-
-  uint4 raw[VPT];
-  if constexpr (!INPLACE) {
-#pragma unroll
-    for (int i = 0; i < VPT; i++) raw[i] = load_row_vec(in, shift, A.V, k0 + i * kRulesThreads);
-  }
-
-  // the tile's mask bits, moved so that bit j of word i is column c0 + 32 i + j
+  const int all = (A.V + shift + N - 1) / N;
+  const int k0 = min(part * A.span, all), k1 = min(k0 + A.span, all);
+  if (k0 >= k1) return;
   const uint32_t *m = mask_row(A, row);
-  const int words = (A.V + 31) / 32;
-  for (int i = tid; i < WORDS; i += kRulesThreads) {
-    uint32_t w = 0xFFFFFFFFu;
-    if (m != nullptr) {
-      const int c = c0 + 32 * i;
-      const int at = c >> 5;  // rounds down for the columns before 0 too
-      const uint32_t lo = (at >= 0 && at < words) ? m[at] : 0u;
-      const uint32_t hi = ((c & 31) != 0 && at + 1 < words) ? m[at + 1] : 0u;
-      w = __funnelshift_r(lo, hi, c & 31);
+  if (LISTS && threadIdx.x >= kRulesThreads) {
+    __shared__ __align__(16) Table S;
+    Lists<Ti, To> L(A, row, max(k0 * N - shift, 0), min(k1 * N - shift, A.V));
+    L.build(S);
+    L.gather(S, in, m);
+    __syncthreads();  // the pass is through
+    L.scatter(S, out);
+    while (L.advance()) {
+      L.sync();
+      L.build(S);
+      L.gather(S, in, m);
+      L.scatter(S, out);
     }
-    s_allow[i] = w;
-    if constexpr (LISTS) s_touch[i] = 0u;
+    return;
   }
-  RowPlan P{};
-  int32_t *s_cnt = s_dyn;
-  int32_t *s_last = s_dyn + (A.hist ? TILE : 0);
-  if constexpr (LISTS) {
-    const int n = ((A.hist ? TILE : 0) + (A.bias_ids ? TILE : 0)) / 4;
-    for (int i = tid; i < n; i += kRulesThreads) reinterpret_cast<int4 *>(s_dyn)[i] = make_int4(0, 0, 0, 0);
-    __syncthreads();
-    if (A.hist != nullptr) {
-      P = plan_row(A.cfg[row], A.V);
-      const int h0 = A.hist_off[row], h1 = P.pen_on ? A.hist_off[row + 1] : h0;
-      for (int64_t j = static_cast<int64_t>(h0) + tid; j < h1; j += kRulesThreads) {
-        const int t = A.hist[j];
-        const int u = t - c0;
-        if (t >= 0 && t < A.V && u >= 0 && u < TILE) {
-          atomicAdd(&s_cnt[u], 1);
-          atomicOr(&s_touch[u >> 5], 1u << (u & 31));
-        }
-      }
-    }
-    if (A.bias_ids != nullptr) {
-      const int b0 = A.bias_off[row], b1 = A.bias_off[row + 1];
-      for (int64_t j = static_cast<int64_t>(b0) + tid; j < b1; j += kRulesThreads) {
-        const int t = A.bias_ids[j];
-        const int u = t - c0;
-        if (t >= 0 && t < A.V && u >= 0 && u < TILE) {
-          atomicMax(&s_last[u], static_cast<int>(j - b0) + 1);
-          atomicOr(&s_touch[u >> 5], 1u << (u & 31));
-        }
-      }
-    }
-  }
-  __syncthreads();
-
-  constexpr uint32_t ALL = (1u << N) - 1u;
-#pragma unroll
-  for (int i = 0; i < VPT; i++) {
-    const int q = (tid + i * kRulesThreads) * N;  // the vector's first column, from c0
-    const int c = c0 + q;
-    if (c >= A.V) continue;
-    const uint32_t allow = (s_allow[q >> 5] >> (q & 31)) & ALL;
-    uint32_t touch = 0u;
-    if constexpr (LISTS) touch = (s_touch[q >> 5] >> (q & 31)) & allow;
-    uint4 r;
-    if constexpr (INPLACE) {
-      if (allow == ALL && touch == 0u) continue;
-      if (allow != 0u) r = load_row_vec(in, shift, A.V, k0 + i * kRulesThreads);
-    } else {
-      r = raw[i];
-    }
-    float x[N];
-    if (allow != 0u) RowElem<Ti>::unpack(r, x);
-    if constexpr (LISTS) {
-      if (touch != 0u) {
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-          if ((touch >> j) & 1u) {
-            if (A.hist != nullptr) {
-              const int n = s_cnt[q + j];
-              if (n > 0) x[j] = penalize(x[j], n, P);
-            }
-            if (A.bias_ids != nullptr) {
-              const int b = s_last[q + j];
-              if (b > 0) x[j] = __fadd_rn(x[j], A.bias_vals[A.bias_off[row] + b - 1]);
-            }
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < N; j++)
-      if (!((allow >> j) & 1u)) x[j] = __int_as_float(0xFF800000);
-    store_row_vec<N>(out, A.V, c, x, aligned);
-  }
+  const MaskPass<Ti, To, INPLACE, LISTS> pass{
+      in, out, m, A.V, shift, (A.V + 31) / 32, k1, whole_vecs<Ti>(shift, A.V),
+      ((reinterpret_cast<uintptr_t>(out) - static_cast<uintptr_t>(shift) * sizeof(To)) & 15u) == 0};
+  pass.run(k0);
+  if (LISTS) __syncthreads();
 }
 
-template <typename Ti, typename To, int VPT, bool INPLACE>
-cudaError_t launch_tiles(RulesArgs &A, int B, cudaStream_t st) {
-  constexpr int N = RowElem<Ti>::N;
-  constexpr int TILE = kRulesThreads * VPT * N;
-  A.tiles = static_cast<int>((static_cast<int64_t>(A.V) + N - 1 + TILE - 1) / TILE);
-  const int64_t ctas = static_cast<int64_t>(B) * (A.tiles + (A.n_allowed != nullptr ? 1 : 0));
-  if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-  const size_t smem = sizeof(int32_t) * TILE * ((A.hist ? 1 : 0) + (A.bias_ids ? 1 : 0));
-  if (smem > 0)
-    rules_kernel<Ti, To, VPT, INPLACE, true><<<static_cast<unsigned>(ctas), kRulesThreads, smem, st>>>(A);
-  else
-    rules_kernel<Ti, To, VPT, INPLACE, false><<<static_cast<unsigned>(ctas), kRulesThreads, 0, st>>>(A);
-  return cudaGetLastError();
-}
-
-// Tiles of 4096 columns; of one vector per thread while the larger ones
-// would leave SMs without a CTA.
+// Parts of a row: 64 KB (1024 rows of 128256 f32 with history, biases and
+// masks: 228 us at 32 KB, 202 at 64 KB, 205 at 128 KB; a row per CTA, a
+// thousand streams apart from one another, 264), smaller ones, of at least
+// one vector per thread, while they would not fill the GPU's CTA slots.
+constexpr int kPartVecs = 4096;
 template <typename Ti, typename To, bool INPLACE>
 cudaError_t launch_rules(RulesArgs &A, int B, cudaStream_t st) {
-  constexpr int VPT = 4096 / (kRulesThreads * RowElem<Ti>::N);
-  if (static_cast<int64_t>(B) * ((A.V + 4095) / 4096) < 2 * current_sms())
-    return launch_tiles<Ti, To, 1, INPLACE>(A, B, st);
-  return launch_tiles<Ti, To, VPT, INPLACE>(A, B, st);
+  constexpr int N = RowElem<Ti>::N;
+  const bool lists = A.hist != nullptr || A.bias_ids != nullptr;
+  const int vecs = (A.V + 2 * N - 2) / N;  // of a row with the largest shift
+  int parts = (vecs + kPartVecs - 1) / kPartVecs;
+  const int most = (vecs + kRulesThreads - 1) / kRulesThreads, wave = current_sms() * 6 / B;
+  if (parts < wave) parts = wave < most ? wave : most;
+  A.parts = parts;
+  A.span = (vecs + parts - 1) / parts;
+  const int64_t ctas = static_cast<int64_t>(B) * (parts + (A.n_allowed != nullptr ? 1 : 0));
+  if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+  if (lists)
+    rules_kernel<Ti, To, INPLACE, true><<<static_cast<unsigned>(ctas), kRulesThreads + kListThreads, 0, st>>>(A);
+  else
+    rules_kernel<Ti, To, INPLACE, false><<<static_cast<unsigned>(ctas), kRulesThreads, 0, st>>>(A);
+  return cudaGetLastError();
 }
 
 }  // namespace
