@@ -170,7 +170,9 @@ struct TcArgs {
   int nt;          // tokens per tile, a multiple of 16
   int tok_tiles;
   int tiles;       // channel tiles x tok_tiles
-  int k_blocks;    // stages' worth of K
+  int k_blocks;    // K in blocks of kTcK
+  int sub;         // blocks per stage
+  int k_stages;    // stages' worth of K
   int k_steps;     // K in steps of 32
   int stages;
   int cols;        // tensor memory columns, a power of two >= 2 nt
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t ring = (smem_addr(s_raw) + 1023u) & ~1023u;
   const uint32_t w_bytes = kTcChannels * kTcK, a_bytes = static_cast<uint32_t>(A.nt) * kTcK;
-  const uint32_t stage_bytes = w_bytes + a_bytes;
+  const uint32_t block_bytes = w_bytes + a_bytes, stage_bytes = block_bytes * A.sub;
   const uint32_t full = smem_addr(s_full), empty = smem_addr(s_empty), sum = smem_addr(s_sum), free_ = smem_addr(s_free);
 
   if (tid == 0) {
@@ -215,36 +217,49 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // The weights of the first stages do not depend on what runs before
       // this kernel (the tokens' quantisation): they are on their way first.
       const int mine = (A.tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-      const int64_t total = static_cast<int64_t>(mine) * A.k_blocks;
+      const int64_t total = static_cast<int64_t>(mine) * A.k_stages;
       const int early = static_cast<int>(total < A.stages ? total : A.stages);
-      int it = 0, ph = 0;  // stage and its phase
-      auto weights = [&](int stage, int tile, int kb) {
-        mbar_expect(full + 8 * stage, stage_bytes);
-        tma_load(ring + stage * stage_bytes, &map_w, kb * kTcK, tile / A.tok_tiles * kTcChannels, full + 8 * stage);
+      // (one thread feeds the SM: no division, no address worked out twice
+      // between two loads)
+      auto weights = [&](uint32_t slot, uint32_t bar, int x, int y, int n) {
+        mbar_expect(bar, block_bytes * n);
+        for (int b = 0; b < n; b++, slot += block_bytes, x += kTcK) tma_load(slot, &map_w, x, y, bar);
       };
       {
-        int tile = blockIdx.x, kb = 0;
+        int tile = blockIdx.x, ks = 0, y = tile / A.tok_tiles * kTcChannels;
         for (int i = 0; i < early; i++) {
-          weights(i, tile, kb);
-          if (++kb == A.k_blocks) {
-            kb = 0;
+          weights(ring + i * stage_bytes, full + 8 * i, ks * A.sub * kTcK, y, min(A.sub, A.k_blocks - ks * A.sub));
+          if (++ks == A.k_stages) {
+            ks = 0;
             tile += gridDim.x;
+            y = tile / A.tok_tiles * kTcChannels;
           }
         }
       }
       pdl_wait();
       int64_t n = 0;
+      uint32_t slot = ring, bar = full, gone = empty, ph = 1;
+      const uint32_t ring_end = ring + A.stages * stage_bytes;
       bool ok = true;
       for (int tile = blockIdx.x; ok && tile < A.tiles; tile += gridDim.x) {
-        for (int kb = 0; kb < A.k_blocks; kb++) {
+        const int yw = tile / A.tok_tiles * kTcChannels, ya = tile % A.tok_tiles * A.nt;
+        for (int kb = 0; kb < A.k_blocks; kb += A.sub) {
+          const int blocks = min(A.sub, A.k_blocks - kb);
+          int x = kb * kTcK;
           if (n >= early) {
-            if (!(ok = mbar_wait(empty + 8 * it, ph ^ 1, &s_stop))) break;
-            weights(it, tile, kb);
+            if (!(ok = mbar_wait(gone, ph, &s_stop))) break;
+            weights(slot, bar, x, yw, blocks);
           }
-          tma_load(ring + it * stage_bytes + w_bytes, &map_a, kb * kTcK, tile % A.tok_tiles * A.nt, full + 8 * it);
+          uint32_t to = slot + w_bytes;
+          for (int b = 0; b < blocks; b++, to += block_bytes, x += kTcK) tma_load(to, &map_a, x, ya, bar);
           n++;
-          if (++it == A.stages) {
-            it = 0;
+          slot += stage_bytes;
+          bar += 8;
+          gone += 8;
+          if (slot == ring_end) {
+            slot = ring;
+            bar = full;
+            gone = empty;
             ph ^= 1;
           }
         }
@@ -262,22 +277,42 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t inst = i8_instruction(A.nt);
-      int it = 0, ph = 0, t = 0;
+      const int whole = A.k_steps / (kTcK / 32);  // blocks of four steps; the last may have fewer
+      const uint64_t block_desc = block_bytes >> 4, a_desc = w_bytes >> 4;
+      uint64_t dw = smem_desc(ring);
+      const uint64_t dw_end = dw + static_cast<uint64_t>(A.stages) * (stage_bytes >> 4);
+      uint32_t bar = full, gone = empty, ph = 0;
+      int t = 0;
       bool ok = true;
       for (int tile = blockIdx.x; ok && tile < A.tiles; tile += gridDim.x, t++) {
         const int acc = t & 1;
         if (!(ok = mbar_wait(free_ + 8 * acc, ((t >> 1) & 1) ^ 1, &s_stop))) break;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(acc * (A.cols / 2));
-        for (int kb = 0; kb < A.k_blocks; kb++) {
-          if (!(ok = mbar_wait(full + 8 * it, ph, &s_stop))) break;
+        bool add = false;
+        for (int kb = 0; kb < A.k_blocks; kb += A.sub) {
+          if (!(ok = mbar_wait(bar, ph, &s_stop))) break;
           tc_fence_after();
-          const uint64_t dw = smem_desc(ring + it * stage_bytes), da = smem_desc(ring + it * stage_bytes + w_bytes);
-          const int steps = min(kTcK / 32, A.k_steps - kb * (kTcK / 32));
-          for (int k = 0; k < steps; k++) tc_mma_i8(d, dw + 2 * k, da + 2 * k, inst, kb > 0 || k > 0);
-          tc_commit(empty + 8 * it);
-          if (++it == A.stages) {
-            it = 0;
+          const int blocks = min(A.sub, A.k_blocks - kb);
+          uint64_t w = dw;
+          for (int b = 0; b < blocks; b++, w += block_desc) {
+            if (kb + b < whole) {
+#pragma unroll
+              for (int k = 0; k < kTcK / 32; k++) tc_mma_i8(d, w + 2 * k, w + a_desc + 2 * k, inst, add || k > 0);
+            } else {
+              for (int k = 0; k < A.k_steps - (kb + b) * (kTcK / 32); k++)
+                tc_mma_i8(d, w + 2 * k, w + a_desc + 2 * k, inst, add || k > 0);
+            }
+            add = true;
+          }
+          tc_commit(gone);
+          dw += stage_bytes >> 4;
+          bar += 8;
+          gone += 8;
+          if (dw == dw_end) {
+            dw = smem_desc(ring);
+            bar = full;
+            gone = empty;
             ph ^= 1;
           }
         }
@@ -400,7 +435,15 @@ cudaError_t launch_matmul_as(const MatmulArgs &P, bool after_quantize, cudaStrea
   A.tiles = static_cast<int>(tiles);
   A.k_blocks = (P.K + kTcK - 1) / kTcK;
   A.k_steps = (P.K + 31) / 32;
-  const int stage = (kTcChannels + A.nt) * kTcK;
+  // Stages of up to a third of the ring: with few tokens, several blocks of K
+  // of the same rows at a time, since 128 bytes here and there is slow from
+  // HBM (1 token, dim 2560, 128256 channels: 58.6 us at one block a stage,
+  // 55.4 at three; 64 tokens, dim 4096, 151936 channels: 127 at one, 116 at
+  // two, 123 at three).
+  const int block = (kTcChannels + A.nt) * kTcK;
+  A.sub = kTcRing / 3 / block;
+  A.k_stages = (A.k_blocks + A.sub - 1) / A.sub;
+  const int stage = block * A.sub;
   A.stages = kTcRing / stage < kTcMaxStages ? kTcRing / stage : kTcMaxStages;
   A.cols = 64;  // (the epilogue reads 32 columns at a time)
   while (A.cols < 2 * A.nt) A.cols *= 2;
