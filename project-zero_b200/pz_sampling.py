@@ -643,42 +643,58 @@ def configs_to_device(cfg_np, device="cuda"):
 # --------------------------------------------------------------------------
 # Rows of logits outside the sampler: constraints, distillation.
 # --------------------------------------------------------------------------
-def _call(fn, name, t, stream, *args):
-    """Calls a context-free entry on t's device, on `stream` or that device's
-    current stream."""
+# (these run at every call of a decode step: indexes instead of device objects,
+# and the raw stream where torch hands it out)
+_raw_stream = None
+
+
+def _current_raw_stream(dev):
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(dev)
+
+
+def _call(fn, name, dev, stream, *args):
+    """Calls a context-free entry on device `dev`, on `stream` or that
+    device's current stream."""
     import torch
-    dev = t.device.index
+    handle = _current_raw_stream(dev) if stream is None else _stream_handle(stream)
     if dev == torch.cuda.current_device():
-        st = fn(*args, torch.cuda.current_stream().cuda_stream if stream is None else _stream_handle(stream))
+        st = fn(*args, handle)
     else:
         with torch.cuda.device(dev):
-            st = fn(*args, torch.cuda.current_stream().cuda_stream if stream is None else _stream_handle(stream))
+            st = fn(*args, handle)
     if st != PZ_OK:
         raise PZError(st, name)
 
 
 def _rows(t, name, like=None):
-    """Checks a [rows, columns] CUDA tensor whose columns are contiguous."""
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{name} has to be [rows, columns] with contiguous columns")
+    """Checks a [rows, columns] CUDA tensor whose columns are contiguous (of
+    the shape and on the device of `like`); its shape and row stride (a single
+    row's may be anything)."""
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name} has to be [rows, columns]")
+    rows, cols = shape
+    ld, step = t.stride()
+    if step != 1 and cols > 1:
+        raise ValueError(f"{name} has to have contiguous columns")
     if not t.is_cuda:
         raise ValueError(f"{name} has to be a CUDA tensor")
-    if like is not None and (t.shape != like.shape or t.device != like.device):
+    if like is not None and (shape != like.shape or t.get_device() != like.get_device()):
         raise ValueError(f"{name} needs the shape and device of the logits")
-    return t
+    return rows, cols, (ld if rows > 1 or ld > cols else cols)
 
 
-def _ld(t):
-    """Elements between rows (a single row's stride may be anything)."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
-
-
-def _vector(t, name, n, dtype, like):
+def _vector(t, name, n, dtype, dev):
     """Checks an optional contiguous vector of at least n elements; its
     device pointer."""
     if t is None:
         return None
-    if t.dtype != dtype or t.numel() < n or not t.is_contiguous() or t.device != like.device:
+    if t.dtype is not dtype or t.get_device() != dev or t.numel() < n or not t.is_contiguous():
         raise ValueError(f"{name} has to be contiguous {dtype} of at least {n} elements on the logits' device")
     return t.data_ptr()
 
@@ -693,61 +709,70 @@ def process_logits(logits, out=None, *, cfg=None, hist=None, hist_off=None, bias
     where the logits are bfloat16.  n_allowed: [B] int32, the ids each row's
     mask leaves.  Returns out."""
     import torch
-    _rows(logits, "logits")
-    B, V = logits.shape
-    if out is None:
-        out = logits
-    else:
-        _rows(out, "out", logits)
     i32 = torch.int32
-    if cfg is not None and (cfg.numel() * cfg.element_size() < 32 * B or not cfg.is_contiguous()
-                            or cfg.device != logits.device):
-        raise ValueError("cfg has to hold one pz_sampler_config (32 bytes) per row on the logits' device")
-    # (an empty tensor has no address: lists without an entry are no lists)
-    if hist is not None and hist.numel() == 0:
-        hist = hist_off = None
-    if bias_ids is not None and bias_ids.numel() == 0:
-        bias_ids = bias_vals = bias_off = None
-    rules = LogitsRules(_ptr(cfg), _vector(hist, "hist", 0, i32, logits),
-                        _vector(hist_off, "hist_off", B + 1, i32, logits),
-                        _vector(bias_ids, "bias_ids", 0, i32, logits),
-                        _vector(bias_vals, "bias_vals", 0, torch.float32, logits),
-                        _vector(bias_off, "bias_off", B + 1, i32, logits))
-    if mask is not None:
-        _rows(mask, "mask")
-        if mask.dtype not in (i32, torch.uint32) or mask.device != logits.device:
-            raise ValueError("mask has to be int32 or uint32 words on the logits' device")
-        rules.mask, rules.mask_ld, rules.mask_rows = mask.data_ptr(), _ld(mask), mask.shape[0]
-        if mask.shape[1] * 32 < V:
-            raise ValueError(f"mask rows of {mask.shape[1]} words do not cover {V} ids")
-        rules.mask_index = _vector(mask_index, "mask_index", B, i32, logits)
-    elif mask_index is not None:
-        raise ValueError("mask_index without mask")
+    B, V, ld = _rows(logits, "logits")
+    dev = logits.get_device()
+    if out is None:
+        out, ld_out = logits, ld
+    else:
+        _, _, ld_out = _rows(out, "out", logits)
     if V == 0:
         raise ValueError("logits without columns")
+    rules = LogitsRules()
+    # (an empty tensor has no address: lists without an entry are no lists)
+    if hist is not None and hist.numel():
+        rules.hist = _vector(hist, "hist", 0, i32, dev)
+        rules.hist_off = _vector(hist_off, "hist_off", B + 1, i32, dev)
+        if cfg is not None:
+            if cfg.numel() * cfg.element_size() < 32 * B or not cfg.is_contiguous() or cfg.get_device() != dev:
+                raise ValueError("cfg has to hold one pz_sampler_config (32 bytes) per row on the logits' device")
+            rules.cfg = cfg.data_ptr()
+    if bias_ids is not None and bias_ids.numel():
+        rules.bias_ids = _vector(bias_ids, "bias_ids", 0, i32, dev)
+        rules.bias_vals = _vector(bias_vals, "bias_vals", bias_ids.numel(), torch.float32, dev)
+        rules.bias_off = _vector(bias_off, "bias_off", B + 1, i32, dev)
+    if mask is not None:
+        rows, words, mask_ld = _rows(mask, "mask")
+        if mask.dtype not in (i32, torch.uint32) or mask.get_device() != dev:
+            raise ValueError("mask has to be int32 or uint32 words on the logits' device")
+        if words * 32 < V:
+            raise ValueError(f"mask rows of {words} words do not cover {V} ids")
+        rules.mask, rules.mask_ld, rules.mask_rows = mask.data_ptr(), mask_ld, rows
+        rules.mask_index = _vector(mask_index, "mask_index", B, i32, dev)
+    elif mask_index is not None:
+        raise ValueError("mask_index without mask")
+    n_out = _vector(n_allowed, "n_allowed", B, i32, dev)
     if B == 0:
         return out
-    _call(_lib.pz_process_logits, "pz_process_logits", logits, stream, logits.data_ptr(), Sampler._dtype_code(logits),
-          B, V, _ld(logits), ctypes.byref(rules), out.data_ptr(), Sampler._dtype_code(out), _ld(out),
-          _vector(n_allowed, "n_allowed", B, i32, logits))
+    _call(_lib.pz_process_logits, "pz_process_logits", dev, stream, logits.data_ptr(), Sampler._dtype_code(logits),
+          B, V, ld, ctypes.byref(rules), out.data_ptr(), Sampler._dtype_code(out), ld_out, n_out)
     return out
 
 
 def _target(logits, ids, values, weight, temperature, mode, n_list):
+    """The checked arguments that the distillation calls share: rows, columns,
+    row stride and device of the logits, and the target."""
     import torch
-    _rows(logits, "logits")
-    _rows(ids, "ids")
-    _rows(values, "values")
-    N = logits.shape[0]
-    if ids.dtype != torch.int32 or values.dtype != torch.float32:
+    N, V, ld = _rows(logits, "logits")
+    dev = logits.get_device()
+    rows, K, ld_ids = _rows(ids, "ids")
+    _, _, ld_values = _rows(values, "values", ids)
+    if ids.dtype is not torch.int32 or values.dtype is not torch.float32:
         raise TypeError("ids have to be int32 and values float32")
-    if ids.shape != values.shape or ids.shape[0] != N or ids.device != logits.device or values.device != ids.device:
+    if rows != N or ids.get_device() != dev:
         raise ValueError("ids and values have to be [rows of the logits, K] on the logits' device")
-    if logits.shape[1] == 0:
+    if V == 0:
         raise ValueError("logits without columns")
-    return DistillTarget(ids.data_ptr(), values.data_ptr(), _ld(ids), _ld(values), ids.shape[1], mode,
-                         _vector(n_list, "n_list", N, torch.int32, logits),
-                         _vector(weight, "weight", N, torch.float32, logits), temperature, 0)
+    return N, V, ld, dev, DistillTarget(ids.data_ptr(), values.data_ptr(), ld_ids, ld_values, K, mode,
+                                        _vector(n_list, "n_list", N, torch.int32, dev),
+                                        _vector(weight, "weight", N, torch.float32, dev), temperature, 0)
+
+
+def _gradient(logits, grad):
+    """Checks the gradient's tensor; its row stride."""
+    if grad.dtype is not logits.dtype:
+        raise TypeError("grad needs the logits' type")
+    return _rows(grad, "grad", logits)[2]
 
 
 def distill_forward(logits, ids, values, loss, stats=None, *, weight=None, temperature=1.0, mode=DISTILL_LIST,
@@ -757,13 +782,12 @@ def distill_forward(logits, ids, values, loss, stats=None, *, weight=None, tempe
     (mode DISTILL_LIST or DISTILL_REST), and, for distill_backward, stats
     [N, 4] float32.  Returns loss."""
     import torch
-    target = _target(logits, ids, values, weight, temperature, mode, n_list)
-    N, V = logits.shape
+    N, V, ld, dev, target = _target(logits, ids, values, weight, temperature, mode, n_list)
+    out = _vector(loss, "loss", N, torch.float32, dev), _vector(stats, "stats", 4 * N, torch.float32, dev)
     if N == 0:
         return loss
-    _call(_lib.pz_distill_forward, "pz_distill_forward", logits, stream, logits.data_ptr(),
-          Sampler._dtype_code(logits), N, V, _ld(logits), ctypes.byref(target),
-          _vector(loss, "loss", N, torch.float32, logits), _vector(stats, "stats", 4 * N, torch.float32, logits))
+    _call(_lib.pz_distill_forward, "pz_distill_forward", dev, stream, logits.data_ptr(), Sampler._dtype_code(logits),
+          N, V, ld, ctypes.byref(target), *out)
     return loss
 
 
@@ -773,17 +797,13 @@ def distill_backward(logits, ids, values, stats, grad, grad_loss=None, *, weight
     themselves) of sum(grad_loss * loss) from distill_forward's stats on the
     same arguments.  Returns grad."""
     import torch
-    target = _target(logits, ids, values, weight, temperature, mode, n_list)
-    N, V = logits.shape
-    _rows(grad, "grad", logits)
-    if grad.dtype != logits.dtype:
-        raise TypeError("grad needs the logits' type")
+    N, V, ld, dev, target = _target(logits, ids, values, weight, temperature, mode, n_list)
+    ld_grad = _gradient(logits, grad)
+    given = _vector(stats, "stats", 4 * N, torch.float32, dev), _vector(grad_loss, "grad_loss", N, torch.float32, dev)
     if N == 0:
         return grad
-    _call(_lib.pz_distill_backward, "pz_distill_backward", logits, stream, logits.data_ptr(),
-          Sampler._dtype_code(logits), N, V, _ld(logits), ctypes.byref(target),
-          _vector(stats, "stats", 4 * N, torch.float32, logits),
-          _vector(grad_loss, "grad_loss", N, torch.float32, logits), grad.data_ptr(), _ld(grad))
+    _call(_lib.pz_distill_backward, "pz_distill_backward", dev, stream, logits.data_ptr(),
+          Sampler._dtype_code(logits), N, V, ld, ctypes.byref(target), *given, grad.data_ptr(), ld_grad)
     return grad
 
 
@@ -793,16 +813,13 @@ def distill_loss_grad(logits, ids, values, loss, grad, *, weight=None, temperatu
     pass over the logits (grad may be the logits themselves).  Returns
     (loss, grad)."""
     import torch
-    target = _target(logits, ids, values, weight, temperature, mode, n_list)
-    N, V = logits.shape
-    _rows(grad, "grad", logits)
-    if grad.dtype != logits.dtype:
-        raise TypeError("grad needs the logits' type")
+    N, V, ld, dev, target = _target(logits, ids, values, weight, temperature, mode, n_list)
+    ld_grad = _gradient(logits, grad)
+    out = _vector(loss, "loss", N, torch.float32, dev)
     if N == 0:
         return loss, grad
-    _call(_lib.pz_distill_loss_grad, "pz_distill_loss_grad", logits, stream, logits.data_ptr(),
-          Sampler._dtype_code(logits), N, V, _ld(logits), ctypes.byref(target),
-          _vector(loss, "loss", N, torch.float32, logits), grad.data_ptr(), _ld(grad))
+    _call(_lib.pz_distill_loss_grad, "pz_distill_loss_grad", dev, stream, logits.data_ptr(),
+          Sampler._dtype_code(logits), N, V, ld, ctypes.byref(target), out, grad.data_ptr(), ld_grad)
     return loss, grad
 
 
@@ -852,15 +869,14 @@ def distill_loss(logits, ids, values, *, weight=None, temperature=1.0, mode=DIST
 # --------------------------------------------------------------------------
 # The LM head in 8-bit integers.
 # --------------------------------------------------------------------------
-def _i8(t, name, like, shape):
-    """Checks an int8 [rows, columns] tensor whose rows start on 16 bytes;
-    its row stride."""
+def _i8(t, name, dev, rows, cols):
+    """Checks an int8 [rows, cols] tensor; its row stride (of a single row
+    any: the library wants a multiple of 16)."""
     import torch
-    _rows(t, name)
-    if t.dtype != torch.int8 or tuple(t.shape) != shape or t.device != like.device:
-        raise ValueError(f"{name} has to be int8 {list(shape)} on the same device")
-    # (a single row's stride is free; the library wants a multiple of 16)
-    return (t.shape[1] + 15) // 16 * 16 if t.shape[0] <= 1 else t.stride(0)
+    r, c, ld = _rows(t, name)
+    if t.dtype is not torch.int8 or r != rows or c != cols or t.get_device() != dev:
+        raise ValueError(f"{name} has to be int8 [{rows}, {cols}] on the same device")
+    return (c + 15) // 16 * 16 if r <= 1 else ld
 
 
 def quantize_rows_i8(x, q, scale, stream=None):
@@ -869,14 +885,14 @@ def quantize_rows_i8(x, q, scale, stream=None):
     (cols + 15) // 16 * 16, dtype=torch.int8)[:, :cols]) and scale [rows]
     float32.  Returns (q, scale)."""
     import torch
-    _rows(x, "x")
-    rows, cols = x.shape
-    ld_q = _i8(q, "q", x, (rows, cols))
-    out = _vector(scale, "scale", rows, torch.float32, x)
+    rows, cols, ld = _rows(x, "x")
+    dev = x.get_device()
+    ld_q = _i8(q, "q", dev, rows, cols)
+    out = _vector(scale, "scale", rows, torch.float32, dev)
     if rows == 0:
         return q, scale
-    _call(_lib.pz_quantize_rows_i8, "pz_quantize_rows_i8", x, stream, x.data_ptr(), Sampler._dtype_code(x), rows,
-          cols, _ld(x), q.data_ptr(), ld_q, out)
+    _call(_lib.pz_quantize_rows_i8, "pz_quantize_rows_i8", dev, stream, x.data_ptr(), Sampler._dtype_code(x), rows,
+          cols, ld, q.data_ptr(), ld_q, out)
     return q, scale
 
 
@@ -884,15 +900,15 @@ def matmul_i8(a, a_scale, w, w_scale, out, stream=None):
     """pz_matmul_i8: out [M, N] (float32 or bfloat16) = (a [M, K] @ w [N, K]^T)
     * a_scale [M] * w_scale [N], the sums in 32-bit integers.  Returns out."""
     import torch
-    _rows(out, "out")
-    M, N = out.shape
-    K = a.shape[1]
-    ld_a, ld_w = _i8(a, "a", out, (M, K)), _i8(w, "w", out, (N, K))
-    sa, sw = (_vector(t, n, k, torch.float32, out) for t, n, k in ((a_scale, "a_scale", M), (w_scale, "w_scale", N)))
+    M, N, ld = _rows(out, "out")
+    dev = out.get_device()
+    K = a.shape[-1]
+    ld_a, ld_w = _i8(a, "a", dev, M, K), _i8(w, "w", dev, N, K)
+    scales = (_vector(a_scale, "a_scale", M, torch.float32, dev), _vector(w_scale, "w_scale", N, torch.float32, dev))
     if M == 0:
         return out
-    _call(_lib.pz_matmul_i8, "pz_matmul_i8", out, stream, a.data_ptr(), ld_a, sa, M, w.data_ptr(), ld_w, sw, N, K,
-          out.data_ptr(), Sampler._dtype_code(out), _ld(out))
+    _call(_lib.pz_matmul_i8, "pz_matmul_i8", dev, stream, a.data_ptr(), ld_a, scales[0], M, w.data_ptr(), ld_w,
+          scales[1], N, K, out.data_ptr(), Sampler._dtype_code(out), ld)
     return out
 
 
@@ -902,18 +918,17 @@ def lm_head_i8(hidden, w_q, w_scale, logits, hidden_q, hidden_scale, stream=None
     int8 / hidden_scale [B], times the classifier w_q [V, dim] int8 with
     w_scale [V] (quantize_rows_i8).  Returns logits."""
     import torch
-    _rows(hidden, "hidden")
-    _rows(logits, "logits")
-    B, dim = hidden.shape
-    V = w_q.shape[0]
-    if tuple(logits.shape) != (B, V) or logits.device != hidden.device:
+    B, dim, ld_hidden = _rows(hidden, "hidden")
+    rows, V, ld = _rows(logits, "logits")
+    dev = hidden.get_device()
+    if rows != B or logits.get_device() != dev:
         raise ValueError("logits have to be [B, V] on the hidden rows' device")
-    ld_w, ld_q = _i8(w_q, "w_q", hidden, (V, dim)), _i8(hidden_q, "hidden_q", hidden, (B, dim))
-    sw, sq = (_vector(t, n, k, torch.float32, hidden)
-              for t, n, k in ((w_scale, "w_scale", V), (hidden_scale, "hidden_scale", B)))
+    ld_w, ld_q = _i8(w_q, "w_q", dev, V, dim), _i8(hidden_q, "hidden_q", dev, B, dim)
+    scales = (_vector(w_scale, "w_scale", V, torch.float32, dev),
+              _vector(hidden_scale, "hidden_scale", B, torch.float32, dev))
     if B == 0:
         return logits
-    _call(_lib.pz_lm_head_logits_i8, "pz_lm_head_logits_i8", hidden, stream, hidden.data_ptr(),
-          Sampler._dtype_code(hidden), B, dim, _ld(hidden), w_q.data_ptr(), ld_w, sw, V, logits.data_ptr(),
-          Sampler._dtype_code(logits), _ld(logits), hidden_q.data_ptr(), ld_q, sq)
+    _call(_lib.pz_lm_head_logits_i8, "pz_lm_head_logits_i8", dev, stream, hidden.data_ptr(),
+          Sampler._dtype_code(hidden), B, dim, ld_hidden, w_q.data_ptr(), ld_w, scales[0], V, logits.data_ptr(),
+          Sampler._dtype_code(logits), ld, hidden_q.data_ptr(), ld_q, scales[1])
     return logits
