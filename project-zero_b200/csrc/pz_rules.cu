@@ -119,13 +119,13 @@ struct Lists {
       const int from = A.hist_off[row], to = A.hist_off[row + 1];
       P = plan_row(A.cfg[row], A.V);
       hist = A.hist + from;
-      n_hist = P.pen_on ? to - from : 0;
+      n_hist = P.pen_on ? max(to - from, 0) : 0;
     }
     if (A.bias_ids != nullptr) {
       const int from = A.bias_off[row];
       bias_ids = A.bias_ids + from;
       bias_vals = A.bias_vals + from;
-      n_bias = A.bias_off[row + 1] - from;
+      n_bias = max(A.bias_off[row + 1] - from, 0);
     }
   }
   static __device__ __forceinline__ uint32_t hash(int id) {  // odd factor: one to one
@@ -134,18 +134,28 @@ struct Lists {
   // The threads that work on the lists, and their barrier.
   static __device__ __forceinline__ int self() { return static_cast<int>(threadIdx.x) - kRulesThreads; }
   static __device__ __forceinline__ void sync() { asm volatile("bar.sync 1, %0;" ::"r"(kListThreads) : "memory"); }
-  // One list's ids of the class into the table.
-  template <bool BIAS>
-  __device__ __forceinline__ void fill(Table &S, const int32_t *ids, int n) const {
-    constexpr int G = 8;  // ids in flight
+  // The lists' ids of the class into the table: the history's, then the
+  // biases', as one list, the next round's ids on their way while one round's
+  // are put in.
+  __device__ __forceinline__ void fill(Table &S) const {
+    constexpr int G = 4;  // ids of a round
     const uint32_t low = bits >= 32 ? 0xFFFFFFFFu : (1u << bits) - 1u;
-    for (int64_t j0 = self(); j0 < n; j0 += G * kListThreads) {
-      int id[G];
-#pragma unroll
-      for (int g = 0; g < G; g++) id[g] = j0 + g * kListThreads < n ? ids[j0 + g * kListThreads] : -1;
+    const int64_t n = static_cast<int64_t>(n_hist) + n_bias;
+    auto load = [&](int64_t j0, int *id) {
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        const int t = id[g];
+        const int64_t j = j0 + g * kListThreads;
+        id[g] = j < n_hist ? hist[j] : j < n ? bias_ids[j - n_hist] : -1;
+      }
+    };
+    int now[G], next[G];
+    load(self(), now);
+    for (int64_t j0 = self(); j0 < n; j0 += G * kListThreads) {
+      load(j0 + G * kListThreads, next);
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const int t = now[g];
+        now[g] = next[g];
         if (t < c0 || t >= c1 || (hash(t) & low) != cls) continue;  // (c0 >= 0)
         uint32_t at = hash(t) >> 22;
         static_assert(kSlots == 1 << 10, "the slot is the hash's top 10 bits");
@@ -155,10 +165,11 @@ struct Lists {
           if (was == -1) S.slot[atomicAdd(&S.taken, 1)] = static_cast<uint16_t>(at);
           if (was == -1 || was == t) break;
         }
+        const int64_t j = j0 + g * kListThreads;
         if (tries == kProbes)
           S.full = 1;
-        else if (BIAS)
-          atomicMax(&S.last[at], static_cast<int>(j0) + g * kListThreads + 1);
+        else if (j >= n_hist)
+          atomicMax(&S.last[at], static_cast<int>(j - n_hist) + 1);
         else
           atomicAdd(&S.count[at], 1);
       }
@@ -174,8 +185,7 @@ struct Lists {
       }
       if (self() == 0) S.taken = S.full = 0;
       sync();
-      fill<false>(S, hist, n_hist);
-      fill<true>(S, bias_ids, n_bias);
+      fill(S);
       sync();
       if (!S.full) return;
       bits++;  // half of the class (32 bits leave one id)
