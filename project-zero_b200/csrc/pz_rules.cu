@@ -90,20 +90,29 @@ constexpr int kProbes = 32;      // a longer run of taken slots counts as a full
 constexpr int kRulesBatch = 4;   // vectors that a thread has in flight
 constexpr int kRulesStep = kRulesBatch * kRulesThreads;
 
-constexpr int kListThreads = 64;  // beside the pass's, in a CTA with lists
+// Threads that work on the lists beside the pass's, and the CTAs per SM that
+// go with them.  More of them shorten a CTA's life where the whole batch is
+// one wave of CTAs (64 rows of 151936 bf16, 1024 ids each: 17.6 us with 64,
+// 12.7 with 128), fewer leave room for more passes where it is many (1024
+// rows of 128256 f32: 202 and 216 us).
+constexpr int kManyLists = 128, kFewLists = 64;
+constexpr int rules_ctas(int lt) { return lt == 0 ? 7 : lt == kManyLists ? 4 : 5; }
+constexpr int kQueue = 256;       // of each of their warps
 
+template <int LT>
 struct Table {
   int32_t key[kSlots];    // id or -1
   int32_t count[kSlots];  // occurrences in the history
   int32_t last[kSlots];   // last bias entry + 1
   uint16_t slot[kSlots];  // the taken slots, in the order they were taken
   float value[kSlots];    // by that order: the new value
+  int2 queue[LT / 32][kQueue];  // ids on their way in, with their places in the lists
   int taken;
   int full;
 };
 
 // The lists of a row in the columns [c0, c1).
-template <typename Ti, typename To>
+template <typename Ti, typename To, int LT>
 struct Lists {
   const int32_t *hist, *bias_ids;  // of this row
   const float *bias_vals;
@@ -133,52 +142,74 @@ struct Lists {
   }
   // The threads that work on the lists, and their barrier.
   static __device__ __forceinline__ int self() { return static_cast<int>(threadIdx.x) - kRulesThreads; }
-  static __device__ __forceinline__ void sync() { asm volatile("bar.sync 1, %0;" ::"r"(kListThreads) : "memory"); }
+  static __device__ __forceinline__ void sync() { asm volatile("bar.sync 1, %0;" ::"r"(LT) : "memory"); }
+  // The first n ids of the warp's queue into the table.
+  __device__ __forceinline__ void insert(Table<LT> &S, const int2 *queue, int n) const {
+    __syncwarp();
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+      const int2 e = queue[i];
+      uint32_t at = hash(e.x) >> 22;
+      static_assert(kSlots == 1 << 10, "the slot is the hash's top 10 bits");
+      int tries = 0;
+      for (; tries < kProbes; tries++, at = (at + 1) % kSlots) {
+        const int was = atomicCAS(&S.key[at], -1, e.x);
+        if (was == -1) S.slot[atomicAdd(&S.taken, 1)] = static_cast<uint16_t>(at);
+        if (was == -1 || was == e.x) break;
+      }
+      if (tries == kProbes)
+        S.full = 1;
+      else if (e.y >= 0)
+        atomicMax(&S.last[at], e.y + 1);
+      else
+        atomicAdd(&S.count[at], 1);
+    }
+    __syncwarp();
+  }
   // The lists' ids of the class into the table: the history's, then the
   // biases', as one list, the next round's ids on their way while one round's
-  // are put in.
-  __device__ __forceinline__ void fill(Table &S) const {
+  // are looked at.  Few lie in the CTA's columns: a warp lines its own up
+  // first, and the table's atomics run with full warps (64 rows with 2048 ids
+  // each: 16.1 us put in as they came, 9.3 lined up).
+  __device__ __forceinline__ void fill(Table<LT> &S) const {
     constexpr int G = 4;  // ids of a round
     const uint32_t low = bits >= 32 ? 0xFFFFFFFFu : (1u << bits) - 1u;
     const int64_t n = static_cast<int64_t>(n_hist) + n_bias;
+    int2 *queue = S.queue[self() >> 5];
     auto load = [&](int64_t j0, int *id) {
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        const int64_t j = j0 + g * kListThreads;
+        const int64_t j = j0 + g * LT + self();
         id[g] = j < n_hist ? hist[j] : j < n ? bias_ids[j - n_hist] : -1;
       }
     };
     int now[G], next[G];
-    load(self(), now);
-    for (int64_t j0 = self(); j0 < n; j0 += G * kListThreads) {
-      load(j0 + G * kListThreads, next);
+    int waiting = 0;
+    load(0, now);
+    for (int64_t j0 = 0; j0 < n; j0 += G * LT) {
+      load(j0 + G * LT, next);
 #pragma unroll
       for (int g = 0; g < G; g++) {
         const int t = now[g];
         now[g] = next[g];
-        if (t < c0 || t >= c1 || (hash(t) & low) != cls) continue;  // (c0 >= 0)
-        uint32_t at = hash(t) >> 22;
-        static_assert(kSlots == 1 << 10, "the slot is the hash's top 10 bits");
-        int tries = 0;
-        for (; tries < kProbes; tries++, at = (at + 1) % kSlots) {
-          const int was = atomicCAS(&S.key[at], -1, t);
-          if (was == -1) S.slot[atomicAdd(&S.taken, 1)] = static_cast<uint16_t>(at);
-          if (was == -1 || was == t) break;
+        const bool here = t >= c0 && t < c1 && (hash(t) & low) == cls;  // (c0 >= 0)
+        const uint32_t all = __ballot_sync(0xFFFFFFFFu, here);
+        if (here) {
+          const int64_t j = j0 + g * LT + self();
+          queue[waiting + __popc(all & lanemask_lt())] = make_int2(t, j < n_hist ? -1 : static_cast<int>(j - n_hist));
         }
-        const int64_t j = j0 + g * kListThreads;
-        if (tries == kProbes)
-          S.full = 1;
-        else if (j >= n_hist)
-          atomicMax(&S.last[at], static_cast<int>(j - n_hist) + 1);
-        else
-          atomicAdd(&S.count[at], 1);
+        waiting += __popc(all);
+      }
+      if (waiting > kQueue - G * 32) {
+        insert(S, queue, waiting);
+        waiting = 0;
       }
     }
+    insert(S, queue, waiting);
   }
   // The next class that fits the table, from the present one on.
-  __device__ __forceinline__ void build(Table &S) {
+  __device__ __forceinline__ void build(Table<LT> &S) {
     for (;;) {
-      for (int i = self(); i < kSlots / 4; i += kListThreads) {
+      for (int i = self(); i < kSlots / 4; i += LT) {
         reinterpret_cast<int4 *>(S.key)[i] = make_int4(-1, -1, -1, -1);
         reinterpret_cast<int4 *>(S.count)[i] = make_int4(0, 0, 0, 0);
         reinterpret_cast<int4 *>(S.last)[i] = make_int4(0, 0, 0, 0);
@@ -203,35 +234,35 @@ struct Lists {
     return true;
   }
   // The new values of the taken slots (a slot whose id the mask takes: none).
-  __device__ __forceinline__ void gather(Table &S, const Ti *in, const uint32_t *m) const {
+  __device__ __forceinline__ void gather(Table<LT> &S, const Ti *in, const uint32_t *m) const {
     constexpr int G = 4;  // loads in flight
     const int n = S.taken;
-    for (int i0 = self(); i0 < n; i0 += G * kListThreads) {
+    for (int i0 = self(); i0 < n; i0 += G * LT) {
       float x[G];
       bool on[G];
 #pragma unroll
       for (int g = 0; g < G; g++) {
         on[g] = false;
-        if (i0 + g * kListThreads < n) {
-          const int t = S.key[S.slot[i0 + g * kListThreads]];
+        if (i0 + g * LT < n) {
+          const int t = S.key[S.slot[i0 + g * LT]];
           x[g] = RowElem<Ti>::get(in + t);
           on[g] = m == nullptr || ((m[t >> 5] >> (t & 31)) & 1u);
         }
       }
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        if (i0 + g * kListThreads >= n) continue;
-        const int at = S.slot[i0 + g * kListThreads];
+        if (i0 + g * LT >= n) continue;
+        const int at = S.slot[i0 + g * LT];
         float y = x[g];
         if (S.count[at] > 0) y = penalize(y, S.count[at], P);
         if (S.last[at] > 0) y = __fadd_rn(y, bias_vals[S.last[at] - 1]);
-        S.value[i0 + g * kListThreads] = y;
+        S.value[i0 + g * LT] = y;
         if (!on[g]) S.key[at] = -1;
       }
     }
   }
-  __device__ __forceinline__ void scatter(const Table &S, To *out) const {
-    for (int i = self(); i < S.taken; i += kListThreads) {
+  __device__ __forceinline__ void scatter(const Table<LT> &S, To *out) const {
+    for (int i = self(); i < S.taken; i += LT) {
       const int t = S.key[S.slot[i]];
       if (t >= 0) RowElem<To>::put(out + t, S.value[i]);
     }
@@ -365,9 +396,9 @@ struct MaskPass {
   }
 };
 
-// kRulesThreads threads for the pass; with lists, kListThreads more.
-template <typename Ti, typename To, bool INPLACE, bool LISTS>
-__global__ void __launch_bounds__(kRulesThreads + (LISTS ? kListThreads : 0), LISTS ? 5 : 7)
+// kRulesThreads threads for the pass and LT for the lists (0: there are none).
+template <typename Ti, typename To, bool INPLACE, int LT>
+__global__ void __launch_bounds__(kRulesThreads + LT, rules_ctas(LT))
     rules_kernel(const RulesArgs A) {
   constexpr int N = RowElem<Ti>::N;
   const int per_row = A.parts + (A.n_allowed != nullptr ? 1 : 0);
@@ -384,26 +415,28 @@ __global__ void __launch_bounds__(kRulesThreads + (LISTS ? kListThreads : 0), LI
   const int k0 = min(part * A.span, all), k1 = min(k0 + A.span, all);
   if (k0 >= k1) return;
   const uint32_t *m = mask_row(A, row);
-  if (LISTS && threadIdx.x >= kRulesThreads) {
-    __shared__ __align__(16) Table S;
-    Lists<Ti, To> L(A, row, max(k0 * N - shift, 0), min(k1 * N - shift, A.V));
-    L.build(S);
-    L.gather(S, in, m);
-    __syncthreads();  // the pass is through
-    L.scatter(S, out);
-    while (L.advance()) {
-      L.sync();
+  if constexpr (LT > 0) {
+    if (threadIdx.x >= kRulesThreads) {
+      __shared__ __align__(16) Table<LT> S;
+      Lists<Ti, To, LT> L(A, row, max(k0 * N - shift, 0), min(k1 * N - shift, A.V));
       L.build(S);
       L.gather(S, in, m);
+      __syncthreads();  // the pass is through
       L.scatter(S, out);
+      while (L.advance()) {
+        L.sync();
+        L.build(S);
+        L.gather(S, in, m);
+        L.scatter(S, out);
+      }
+      return;
     }
-    return;
   }
-  const MaskPass<Ti, To, INPLACE, LISTS> pass{
+  const MaskPass<Ti, To, INPLACE, (LT > 0)> pass{
       in, out, m, A.V, shift, (A.V + 31) / 32, k1, whole_vecs<Ti>(shift, A.V),
       ((reinterpret_cast<uintptr_t>(out) - static_cast<uintptr_t>(shift) * sizeof(To)) & 15u) == 0};
   pass.run(k0);
-  if (LISTS) __syncthreads();
+  if (LT > 0) __syncthreads();
 }
 
 // Parts of a row: 64 KB (1024 rows of 128256 f32 with history, biases and
@@ -417,16 +450,21 @@ cudaError_t launch_rules(RulesArgs &A, int B, cudaStream_t st) {
   const bool lists = A.hist != nullptr || A.bias_ids != nullptr;
   const int vecs = (A.V + 2 * N - 2) / N;  // of a row with the largest shift
   int parts = (vecs + kPartVecs - 1) / kPartVecs;
-  const int most = (vecs + kRulesThreads - 1) / kRulesThreads, wave = current_sms() * 6 / B;
+  const int most = (vecs + kRulesThreads - 1) / kRulesThreads;
+  const int wave = current_sms() * rules_ctas(lists ? kManyLists : 0) / B - (A.n_allowed != nullptr ? 1 : 0);
+  const bool one_wave = parts <= wave;
   if (parts < wave) parts = wave < most ? wave : most;
   A.parts = parts;
   A.span = (vecs + parts - 1) / parts;
   const int64_t ctas = static_cast<int64_t>(B) * (parts + (A.n_allowed != nullptr ? 1 : 0));
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-  if (lists)
-    rules_kernel<Ti, To, INPLACE, true><<<static_cast<unsigned>(ctas), kRulesThreads + kListThreads, 0, st>>>(A);
+  const unsigned grid = static_cast<unsigned>(ctas);
+  if (!lists)
+    rules_kernel<Ti, To, INPLACE, 0><<<grid, kRulesThreads, 0, st>>>(A);
+  else if (one_wave)
+    rules_kernel<Ti, To, INPLACE, kManyLists><<<grid, kRulesThreads + kManyLists, 0, st>>>(A);
   else
-    rules_kernel<Ti, To, INPLACE, false><<<static_cast<unsigned>(ctas), kRulesThreads, 0, st>>>(A);
+    rules_kernel<Ti, To, INPLACE, kFewLists><<<grid, kRulesThreads + kFewLists, 0, st>>>(A);
   return cudaGetLastError();
 }
 
