@@ -296,34 +296,35 @@ struct MaskPass {
     if (off > 32 - N && at + 1 < words) w |= __ldg(m + at + 1) << (32 - off);
     return w & ALL;
   }
-  __device__ __forceinline__ void load(int kb, uint4 *raw, uint32_t *allow) const {
+  // A batch's mask bits (past its end: all, which changes nothing in place).
+  __device__ __forceinline__ void bits(int kb, uint32_t *allow) const {
     const int k = kb + static_cast<int>(threadIdx.x);
-    if (whole_batch(kb)) {
-      const int c = k * N - shift;
-      if (!INPLACE) {
-#pragma unroll
-        for (int i = 0; i < kRulesBatch; i++) raw[i] = load16(in + c + i * kRulesThreads * N);
-      }
-      if (m == nullptr) return;
+    const int c = k * N - shift;
+    if (m == nullptr) return;
+    if (shift == 0 && whole_batch(kb)) {  // one word holds a vector's bits
       const int off = c & 31;
       const uint32_t *p = m + (c >> 5);
-      if (shift == 0) {  // off + N <= 32
 #pragma unroll
-        for (int i = 0; i < kRulesBatch; i++) allow[i] = (__ldg(p + i * WORDS) >> off) & ALL;
-      } else {
-#pragma unroll
-        for (int i = 0; i < kRulesBatch; i++) allow[i] = bits_at(c + i * kRulesThreads * N);
-      }
+      for (int i = 0; i < kRulesBatch; i++) allow[i] = (__ldg(p + i * WORDS) >> off) & ALL;
     } else {
 #pragma unroll
-      for (int i = 0; i < kRulesBatch; i++) {
-        const int v = k + i * kRulesThreads;
-        allow[i] = ALL;
-        if (v < k1) {
-          if (!INPLACE) raw[i] = vec(v);
-          if (m != nullptr) allow[i] = bits_at(v * N - shift);
-        }
-      }
+      for (int i = 0; i < kRulesBatch; i++)
+        allow[i] = k + i * kRulesThreads < k1 ? bits_at(c + i * kRulesThreads * N) : ALL;
+    }
+  }
+  // A batch's vectors; in place only those that keep some of their values.
+  __device__ __forceinline__ void data(int kb, const uint32_t *allow, uint4 *raw) const {
+    const int k = kb + static_cast<int>(threadIdx.x);
+    if (whole_batch(kb)) {
+      const Ti *p = in + (k * N - shift);
+#pragma unroll
+      for (int i = 0; i < kRulesBatch; i++)
+        if (!INPLACE || (allow[i] != ALL && allow[i] != 0u)) raw[i] = load16(p + i * kRulesThreads * N);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRulesBatch; i++)
+        if (k + i * kRulesThreads < k1 && (!INPLACE || (allow[i] != ALL && allow[i] != 0u)))
+          raw[i] = vec(k + i * kRulesThreads);
     }
   }
   __device__ __forceinline__ uint4 vec(int k) const {
@@ -331,11 +332,6 @@ struct MaskPass {
   }
   __device__ __forceinline__ void store(int kb, uint4 *raw, const uint32_t *allow) const {
     const int k = kb + static_cast<int>(threadIdx.x);
-    if (INPLACE) {  // only the vectors that keep some of their values are read
-#pragma unroll
-      for (int i = 0; i < kRulesBatch; i++)
-        if (allow[i] != ALL && allow[i] != 0u) raw[i] = vec(k + i * kRulesThreads);
-    }
     if (m != nullptr) {
 #pragma unroll
       for (int i = 0; i < kRulesBatch; i++) raw[i] = RowElem<Ti>::keep(raw[i], allow[i]);
@@ -379,18 +375,28 @@ struct MaskPass {
       for (int j = 0; j < N; j += RowElem<To>::N) store_edge(out, V, c + j, RowElem<To>::pack(x + j));
     }
   }
-  // The next batch is in flight while one is worked on.
+  // The next batch's vectors are in flight while one is worked on; in place,
+  // where they hang on the mask, the bits of the one after.
   __device__ __forceinline__ void run(int k0) const {
     if (INPLACE && m == nullptr) return;
     uint4 a[kRulesBatch], b[kRulesBatch];
-    uint32_t aa[kRulesBatch], ab[kRulesBatch];
-    load(k0, a, aa);
-    for (int kb = k0; kb < k1; kb += 2 * kRulesStep) {
-      if (kb + kRulesStep < k1) load(kb + kRulesStep, b, ab);
+    uint32_t aa[kRulesBatch], ab[kRulesBatch], ac[kRulesBatch];
+    bits(k0, aa);
+    if (INPLACE && k0 + kRulesStep < k1) bits(k0 + kRulesStep, ab);
+    data(k0, aa, a);
+    for (int kb = k0; kb < k1; kb += kRulesStep) {
+      if (INPLACE) {
+        if (kb + 2 * kRulesStep < k1) bits(kb + 2 * kRulesStep, ac);
+      } else if (kb + kRulesStep < k1) {
+        bits(kb + kRulesStep, ab);
+      }
+      if (kb + kRulesStep < k1) data(kb + kRulesStep, ab, b);
       store(kb, a, aa);
-      if (kb + kRulesStep < k1) {
-        if (kb + 2 * kRulesStep < k1) load(kb + 2 * kRulesStep, a, aa);
-        store(kb + kRulesStep, b, ab);
+#pragma unroll
+      for (int i = 0; i < kRulesBatch; i++) {
+        a[i] = b[i];
+        aa[i] = ab[i];
+        if (INPLACE) ab[i] = ac[i];
       }
     }
   }
