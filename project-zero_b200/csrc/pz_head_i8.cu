@@ -146,16 +146,18 @@ struct MatmulArgs {
 // Warp 0 issues TMA loads (128 channels x 128 bytes of K and the tokens'
 // part, 128-byte swizzle) into a ring of stages; one thread of warp 1 issues
 // four tcgen05.mma (K = 32 each) per stage; the sums lie in tensor memory,
-// two tiles of them, so that warps 2 to 5 read, scale and store one tile
+// two tiles of them, so that the other warps read, scale and store one tile
 // while the next is summed.  A lane of the epilogue holds one channel: a
-// warp stores 32 neighbouring logits of a token at a time.
+// warp stores 32 neighbouring logits of a token at a time.  Eight warps of
+// it: four took 2.9 us for a tile of 160 tokens, as long as K = 2000 of sums.
 //
 // Rows and K past the matrices' ends arrive as zeros.  Every wait is bounded:
 // one that runs out (4 s; nothing in this kernel can cause it) ends the CTA
 // after its loads have landed and its products are done, with NaN in the
 // outputs it did not reach.
 // ---------------------------------------------------------------------------
-constexpr int kTcThreads = 192;
+constexpr int kTcWarps = 8;           // of the epilogue
+constexpr int kTcThreads = 64 + 32 * kTcWarps;
 constexpr int kTcChannels = 128;
 constexpr int kTcTokens = 256;
 constexpr int kTcK = 128;             // bytes of K per stage
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(sum + 8 * i, 1);
-      mbar_init(free_ + 8 * i, 4);
+      mbar_init(free_ + 8 * i, kTcWarps);
     }
     mbar_init(smem_addr(&s_drain), 1);
     mbar_init_fence();
@@ -328,6 +330,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else {
     pdl_wait();
     const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
+    const int first = (warp - 2) / 4 * 32;  // its first token; two warps share a quarter, 32 tokens in turn
     const int row = quarter * 32 + lane;
     int t = 0;
     bool ok = true;
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) {
         for (int j = 0; j < tokens; j++)
-          if (n < A.N) RowElem<T>::put(out + static_cast<int64_t>(j) * A.ld_out, __int_as_float(0x7FC00000));
+          if (n < A.N && first == 0) RowElem<T>::put(out + static_cast<int64_t>(j) * A.ld_out, __int_as_float(0x7FC00000));
         continue;
       }
       tc_fence_after();
@@ -349,13 +352,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t at = tmem + static_cast<uint32_t>(acc * (A.cols / 2)) + (static_cast<uint32_t>(quarter * 32) << 16);
       // 32 tokens at a time; each lane fetches one token's scale, ahead of
       // the stores that the compiler may not move a load across
-      float sa = lane < tokens ? __ldcg(A.a_scale + m0 + lane) : 0.0f;
-      for (int c = 0; c < tokens; c += 32) {
+      float sa = first + lane < tokens ? __ldcg(A.a_scale + m0 + first + lane) : 0.0f;
+      constexpr int STEP = 8 * kTcWarps;
+      for (int c = first; c < tokens; c += STEP) {
         int v[32];
         __syncwarp();
         tmem_load32(at + c, v);
         const float here = sa;
-        if (c + 32 + lane < tokens) sa = __ldcg(A.a_scale + m0 + c + 32 + lane);
+        if (c + STEP + lane < tokens) sa = __ldcg(A.a_scale + m0 + c + STEP + lane);
         tmem_load_wait();
         float x[32];
 #pragma unroll
