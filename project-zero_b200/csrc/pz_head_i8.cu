@@ -139,9 +139,13 @@ struct MatmulArgs {
 // up to 256 tokens (its N, a multiple of 16).
 //
 // Few tokens: bound by HBM, every weight read once: a persistent CTA per SM
-// keeps about 200 KB of weights and tokens in flight.  Many tokens: bound by
-// the tensor cores and, behind them, by L2 (a tile of 128 x 256 reads 384
-// bytes per 32768 products).
+// keeps about 200 KB of weights and tokens in flight (1 token, dim 2560,
+// 128256 channels: 53 us, 6.3 TB/s; 64 tokens, dim 4096, 151936 channels: 108
+// us, 6.1 TB/s).  Many tokens: bound by what the SMs fetch from L2 (54 bytes a
+// clock each, measured; a tile of 128 x 256 wants 384 bytes per 32768
+// products, half a tile in a pair of CTAs 256), and beside it by the tensor
+// cores and the power limit (4096 tokens, dim 4096, 128256 channels: 1.42 to
+// 1.55 ms, 2.8 to 3.0 POP/s).
 //
 // Warp 0 issues TMA loads (128 channels x 128 bytes of K and the tokens'
 // part, 128-byte swizzle) into a ring of stages; one thread of warp 1 issues
@@ -180,7 +184,12 @@ struct TcArgs {
   int cols;        // tensor memory columns, a power of two >= 2 nt
 };
 
-template <typename T>
+// PAIR: clusters of two CTAs (two SMs) sum tiles of 256 channels together,
+// each CTA's 128 from its own weights and tokens that lie half in either's
+// shared memory, so that a CTA reads half as many tokens.  The leading CTA's
+// barriers count both CTAs' loads, it issues the products for both and tells
+// both of their end.
+template <typename T, bool PAIR>
 __global__ void __launch_bounds__(kTcThreads, 1)
     matmul_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const TcArgs A) {
   extern __shared__ unsigned char s_raw[];
@@ -189,7 +198,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ volatile int s_stop;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t ring = (smem_addr(s_raw) + 1023u) & ~1023u;
-  const uint32_t w_bytes = kTcChannels * kTcK, a_bytes = static_cast<uint32_t>(A.nt) * kTcK;
+  const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u;
+  const int tile0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  constexpr int kTileChannels = PAIR ? 2 * kTcChannels : kTcChannels;
+  const int a_rows = PAIR ? A.nt / 2 : A.nt;  // tokens in this CTA's shared memory
+  const uint32_t w_bytes = kTcChannels * kTcK, a_bytes = static_cast<uint32_t>(a_rows) * kTcK;
   const uint32_t block_bytes = w_bytes + a_bytes, stage_bytes = block_bytes * A.sub;
   const uint32_t full = smem_addr(s_full), empty = smem_addr(s_empty), sum = smem_addr(s_sum), free_ = smem_addr(s_free);
 
@@ -202,15 +215,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(sum + 8 * i, 1);
-      mbar_init(free_ + 8 * i, kTcWarps);
+      mbar_init(free_ + 8 * i, PAIR ? 2 * kTcWarps : kTcWarps);
     }
     mbar_init(smem_addr(&s_drain), 1);
     mbar_init_fence();
     s_stop = 0;
   }
-  if (warp == 2) tmem_alloc(smem_addr(&s_tmem), static_cast<uint32_t>(A.cols));
+  if (warp == 2) tmem_alloc<PAIR>(smem_addr(&s_tmem), static_cast<uint32_t>(A.cols));
   tc_fence_before();
   __syncthreads();
+  if (PAIR) pair_sync();  // the other CTA's barriers are set up too
   tc_fence_after();
   const uint32_t tmem = s_tmem;
 
@@ -218,23 +232,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (lane == 0) {
       // The weights of the first stages do not depend on what runs before
       // this kernel (the tokens' quantisation): they are on their way first.
-      const int mine = (A.tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+      const int mine = (A.tiles - tile0 + tile_step - 1) / tile_step;
       const int64_t total = static_cast<int64_t>(mine) * A.k_stages;
       const int early = static_cast<int>(total < A.stages ? total : A.stages);
       // (one thread feeds the SM: no division, no address worked out twice
       // between two loads)
+      const uint32_t lead = PAIR ? remote_addr(full, 0) : full;  // the barriers that count the loads
       auto weights = [&](uint32_t slot, uint32_t bar, int x, int y, int n) {
-        mbar_expect(bar, block_bytes * n);
-        for (int b = 0; b < n; b++, slot += block_bytes, x += kTcK) tma_load(slot, &map_w, x, y, bar);
+        if (rank == 0) mbar_expect(bar, (PAIR ? 2 : 1) * block_bytes * n);
+        for (int b = 0; b < n; b++, slot += block_bytes, x += kTcK)
+          tma_load<PAIR>(slot, &map_w, x, y, bar - full + lead);
       };
       {
-        int tile = blockIdx.x, ks = 0, y = tile / A.tok_tiles * kTcChannels;
+        int tile = tile0, ks = 0, y = tile / A.tok_tiles * kTileChannels + rank * kTcChannels;
         for (int i = 0; i < early; i++) {
           weights(ring + i * stage_bytes, full + 8 * i, ks * A.sub * kTcK, y, min(A.sub, A.k_blocks - ks * A.sub));
           if (++ks == A.k_stages) {
             ks = 0;
-            tile += gridDim.x;
-            y = tile / A.tok_tiles * kTcChannels;
+            tile += tile_step;
+            y = tile / A.tok_tiles * kTileChannels + rank * kTcChannels;
           }
         }
       }
@@ -243,8 +259,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint32_t slot = ring, bar = full, gone = empty, ph = 1;
       const uint32_t ring_end = ring + A.stages * stage_bytes;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < A.tiles; tile += gridDim.x) {
-        const int yw = tile / A.tok_tiles * kTcChannels, ya = tile % A.tok_tiles * A.nt;
+      for (int tile = tile0; ok && tile < A.tiles; tile += tile_step) {
+        const int yw = tile / A.tok_tiles * kTileChannels + rank * kTcChannels;
+        const int ya = tile % A.tok_tiles * A.nt + rank * a_rows;
         for (int kb = 0; kb < A.k_blocks; kb += A.sub) {
           const int blocks = min(A.sub, A.k_blocks - kb);
           int x = kb * kTcK;
@@ -253,7 +270,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             weights(slot, bar, x, yw, blocks);
           }
           uint32_t to = slot + w_bytes;
-          for (int b = 0; b < blocks; b++, to += block_bytes, x += kTcK) tma_load(to, &map_a, x, ya, bar);
+          for (int b = 0; b < blocks; b++, to += block_bytes, x += kTcK)
+            tma_load<PAIR>(to, &map_a, x, ya, bar - full + lead);
           n++;
           slot += stage_bytes;
           bar += 8;
@@ -266,8 +284,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      // after a stop: no load may be in flight when the CTA's memory goes
-      if (s_stop) {
+      // no commit may be on its way to this CTA's barriers when its memory goes
+      for (int64_t i = n < A.stages ? 0 : n - A.stages; ok && PAIR && i < n; i++)
+        ok = mbar_wait(empty + 8 * static_cast<uint32_t>(i % A.stages), static_cast<uint32_t>((i / A.stages) & 1), &s_stop);
+      // after a stop: no load may be in flight when the CTA's memory goes (the
+      // leading CTA waits for both CTAs' loads)
+      if (s_stop && rank == 0) {
         const int64_t last = n < A.stages ? n : A.stages;
         for (int64_t i = n - last; i < n; i++) {
           volatile int ignore = 0;
@@ -277,8 +299,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t inst = i8_instruction(A.nt);
+    if (lane == 0 && rank == 0) {
+      const uint32_t inst = i8_instruction(kTileChannels, A.nt);
       const int whole = A.k_steps / (kTcK / 32);  // blocks of four steps; the last may have fewer
       const uint64_t block_desc = block_bytes >> 4, a_desc = w_bytes >> 4;
       uint64_t dw = smem_desc(ring);
@@ -286,7 +308,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint32_t bar = full, gone = empty, ph = 0;
       int t = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < A.tiles; tile += gridDim.x, t++) {
+      for (int tile = tile0; ok && tile < A.tiles; tile += tile_step, t++) {
         const int acc = t & 1;
         if (!(ok = mbar_wait(free_ + 8 * acc, ((t >> 1) & 1) ^ 1, &s_stop))) break;
         tc_fence_after();
@@ -300,14 +322,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int b = 0; b < blocks; b++, w += block_desc) {
             if (kb + b < whole) {
 #pragma unroll
-              for (int k = 0; k < kTcK / 32; k++) tc_mma_i8(d, w + 2 * k, w + a_desc + 2 * k, inst, add || k > 0);
+              for (int k = 0; k < kTcK / 32; k++) tc_mma_i8<PAIR>(d, w + 2 * k, w + a_desc + 2 * k, inst, add || k > 0);
             } else {
               for (int k = 0; k < A.k_steps - (kb + b) * (kTcK / 32); k++)
-                tc_mma_i8(d, w + 2 * k, w + a_desc + 2 * k, inst, add || k > 0);
+                tc_mma_i8<PAIR>(d, w + 2 * k, w + a_desc + 2 * k, inst, add || k > 0);
             }
             add = true;
           }
-          tc_commit(gone);
+          tc_commit<PAIR>(gone);
           dw += stage_bytes >> 4;
           bar += 8;
           gone += 8;
@@ -318,11 +340,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             ph ^= 1;
           }
         }
-        if (ok) tc_commit(sum + 8 * acc);
+        if (ok) tc_commit<PAIR>(sum + 8 * acc);
       }
       if (s_stop) {
         volatile int ignore = 0;
-        tc_commit(smem_addr(&s_drain));
+        tc_commit<PAIR>(smem_addr(&s_drain));
         mbar_wait(smem_addr(&s_drain), 0, &ignore);
       }
     }
@@ -334,9 +356,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int row = quarter * 32 + lane;
     int t = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < A.tiles; tile += gridDim.x, t++) {
+    const uint32_t freed = PAIR ? remote_addr(free_, 0) : free_;
+    for (int tile = tile0; tile < A.tiles; tile += tile_step, t++) {
       const int acc = t & 1;
-      const int n = tile / A.tok_tiles * kTcChannels + row;
+      const int n = tile / A.tok_tiles * kTileChannels + rank * kTcChannels + row;
       const int m0 = tile % A.tok_tiles * A.nt;
       T *out = static_cast<T *>(A.out) + static_cast<int64_t>(m0) * A.ld_out + n;
       const int tokens = min(A.nt, A.M - m0);
@@ -379,15 +402,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(free_ + 8 * acc);
+      if (lane == 0) PAIR ? mbar_arrive_remote(freed + 8 * acc) : mbar_arrive(freed + 8 * acc);
     }
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) pair_sync();  // neither CTA's memory or barriers are used by the other any more
   if (warp == 2) {
     tc_fence_after();
-    tmem_free(tmem, static_cast<uint32_t>(A.cols));
+    tmem_free<PAIR>(tmem, static_cast<uint32_t>(A.cols));
   }
 }
 
@@ -423,7 +447,7 @@ bool encode_rows(CUtensorMap *map, const int8_t *p, int K, int rows, int64_t ld,
 
 // after_quantize: launched behind the tokens' quantisation, whose end the
 // kernel waits for itself.
-template <typename T>
+template <typename T, bool PAIR>
 cudaError_t launch_matmul_as(const MatmulArgs &P, bool after_quantize, cudaStream_t st) {
   TcArgs A{};
   A.a_scale = P.a_scale;
@@ -432,19 +456,21 @@ cudaError_t launch_matmul_as(const MatmulArgs &P, bool after_quantize, cudaStrea
   A.ld_out = P.ld_out;
   A.M = P.M;
   A.N = P.N;
+  constexpr int UNIT = PAIR ? 32 : 16;  // the instruction's step of tokens
   A.tok_tiles = (P.M + kTcTokens - 1) / kTcTokens;
-  A.nt = ((P.M + A.tok_tiles - 1) / A.tok_tiles + 15) / 16 * 16;
-  const int64_t tiles = static_cast<int64_t>((P.N + kTcChannels - 1) / kTcChannels) * A.tok_tiles;
+  A.nt = ((P.M + A.tok_tiles - 1) / A.tok_tiles + UNIT - 1) / UNIT * UNIT;
+  const int a_rows = PAIR ? A.nt / 2 : A.nt, channels = PAIR ? 2 * kTcChannels : kTcChannels;
+  const int64_t tiles = static_cast<int64_t>((P.N + channels - 1) / channels) * A.tok_tiles;
   if (tiles > 0x3FFFFFFF) return cudaErrorInvalidConfiguration;
   A.tiles = static_cast<int>(tiles);
   A.k_blocks = (P.K + kTcK - 1) / kTcK;
   A.k_steps = (P.K + 31) / 32;
-  // Stages of up to a third of the ring: with few tokens, several blocks of K
-  // of the same rows at a time, since 128 bytes here and there is slow from
-  // HBM (1 token, dim 2560, 128256 channels: 58.6 us at one block a stage,
-  // 55.4 at three; 64 tokens, dim 4096, 151936 channels: 127 at one, 116 at
-  // two, 123 at three).
-  const int block = (kTcChannels + A.nt) * kTcK;
+  // Stages of up to a third of the ring: several blocks of K of the same rows
+  // at a time, since 128 bytes here and there is slow from HBM (1 token, dim
+  // 2560, 128256 channels: 58.6 us at one block a stage, 55.4 at three; 64
+  // tokens, dim 4096, 151936 channels: 127 at one, 116 at two, 123 at three;
+  // 4096 tokens in pairs: 1815 at one, 1523 at two).
+  const int block = (kTcChannels + a_rows) * kTcK;
   A.sub = kTcRing / 3 / block;
   A.k_stages = (A.k_blocks + A.sub - 1) / A.sub;
   const int stage = block * A.sub;
@@ -452,30 +478,48 @@ cudaError_t launch_matmul_as(const MatmulArgs &P, bool after_quantize, cudaStrea
   A.cols = 64;  // (the epilogue reads 32 columns at a time)
   while (A.cols < 2 * A.nt) A.cols *= 2;
   CUtensorMap map_w, map_a;
-  if (!encode_rows(&map_w, P.w, P.K, P.N, P.ld_w, kTcChannels) || !encode_rows(&map_a, P.a, P.K, P.M, P.ld_a, A.nt))
+  if (!encode_rows(&map_w, P.w, P.K, P.N, P.ld_w, kTcChannels) || !encode_rows(&map_a, P.a, P.K, P.M, P.ld_a, a_rows))
     return cudaErrorInvalidValue;
   const size_t smem = static_cast<size_t>(A.stages) * stage + 1024;
   static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
-  cudaError_t e = allow_smem(reinterpret_cast<const void *>(matmul_i8_kernel<T>), kTcRing + 1024, &ready);
+  cudaError_t e = allow_smem(reinterpret_cast<const void *>(matmul_i8_kernel<T, PAIR>), kTcRing + 1024, &ready);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  const int sms = current_sms();
-  cfg.gridDim = dim3(static_cast<unsigned>(A.tiles < sms ? A.tiles : sms));
+  const int groups = current_sms() / (PAIR ? 2 : 1);
+  cfg.gridDim = dim3(static_cast<unsigned>((A.tiles < groups ? A.tiles : groups) * (PAIR ? 2 : 1)));
   cfg.blockDim = dim3(kTcThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (after_quantize) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (PAIR) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = 2;
+    at[n].val.clusterDim.y = 1;
+    at[n++].val.clusterDim.z = 1;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = after_quantize ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, matmul_i8_kernel<T>, map_w, map_a, A);
+  cfg.numAttrs = n;
+  e = cudaLaunchKernelEx(&cfg, matmul_i8_kernel<T, PAIR>, map_w, map_a, A);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+// Pairs from here on (dim 4096, 128256 channels, bf16 logits: 64 tokens 88.8
+// us alone and 88.3 in pairs, 96: 94.0 and 90.9, 256: 132 and 117, 1024: 489
+// and 390; dim 1000, 32003 channels: 64: 11.4 and 11.4, 256: 25.4 and 19.1).
+constexpr int kPairTokens = 65;
+template <typename T>
+cudaError_t launch_matmul_to(const MatmulArgs &A, bool after_quantize, cudaStream_t st) {
+  return A.M >= kPairTokens ? launch_matmul_as<T, true>(A, after_quantize, st)
+                            : launch_matmul_as<T, false>(A, after_quantize, st);
+}
 cudaError_t launch_matmul(const MatmulArgs &A, pz_dtype out_dtype, bool after_quantize, cudaStream_t st) {
-  return out_dtype == PZ_DTYPE_F32 ? launch_matmul_as<float>(A, after_quantize, st)
-                                   : launch_matmul_as<bf16_t>(A, after_quantize, st);
+  return out_dtype == PZ_DTYPE_F32 ? launch_matmul_to<float>(A, after_quantize, st)
+                                   : launch_matmul_to<bf16_t>(A, after_quantize, st);
 }
 
 pz_status check_quantize(const void *x, pz_dtype dtype, int rows, int cols, int64_t ld, const int8_t *q, int64_t ld_q,
