@@ -24,14 +24,22 @@
 // rho / r hold when the student leaves them next to nothing.  The sum over
 // the list, whose terms nearly cancel against log S, is in fp64.
 //
-// Bound: HBM.  The loss reads the logits once; the gradient from saved
-// statistics reads and writes once; loss and gradient together read once and
-// write once, because a row stays on chip between its two passes: a cluster
-// of up to 8 CTAs takes a row, each CTA holding 64 KB of it in registers
-// (512 threads x 8 vectors of 16 bytes, two CTAs per SM), and they exchange
-// maximum and sums through distributed shared memory.  Columns beyond
-// 8 x 64 KB are read a second time (from L2, mostly: the rows in flight are
-// at most 148 x 2 / 8 of them).
+// Bound: HBM, and for bf16 loss and gradient together the SMs' issue slots
+// (two exponentials per id and what every warp repeats per row).
+//   loss      a row per CTA while the rows fill the GPU, parts of one in a
+//             cluster otherwise; the next batch of vectors in flight while one
+//             is summed.  1024 rows of 128256 f32: 77 us, 6.8 TB/s.
+//   gradient  from saved statistics: parts of 64 KB, independent CTAs.  2048
+//             rows of 151936 bf16: 190 us, 6.5 TB/s (after a loss of 99 us).
+//   both      one read and one write: a row stays on chip between its two
+//             passes.  A cluster of up to 8 CTAs takes it, each fetching 32 KB
+//             of it into shared memory (cp.async; a thread reads back what it
+//             fetched itself), and they exchange maximum and sums through
+//             distributed shared memory.  4096 rows of 128256 bf16: 412 us,
+//             5.1 TB/s.  Four warps a CTA: with eight, each repeating the
+//             row's scalars for half as many columns, it was 566 us, with two
+//             495; parts of 64 KB (three CTAs on an SM, not five) 505.
+// The list is read by all parts of its row: at most 1024 ids, two barriers.
 #include <atomic>
 
 #include "pz_device.cuh"
@@ -45,7 +53,7 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;              // 16-byte vectors that a thread works on at a time
 constexpr int kStep = kBatch * kThreads;
-constexpr int kEntries = PZ_TOP_K_MAX / kThreads;  // most list entries of a thread
+constexpr int kEntries = (PZ_TOP_K_MAX + kThreads - 1) / kThreads;  // most list entries of a thread
 constexpr int kFlagWords = 4;
 constexpr int kMaxSpan = kFlagWords * 32 * kStep;   // vectors of a span: a flag per batch of a thread
 constexpr int kMaxCluster = 8;         // the portable cluster size
@@ -444,6 +452,16 @@ struct RowPart {
   }
 };
 
+__device__ __forceinline__ int cluster_rank() {
+  int r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ int cluster_id() {
+  int r;
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(r));
+  return r;
+}
 // The row's cluster: all CTAs have to arrive before any passes the wait.
 // Threads that wrote nothing for the others arrive without a fence.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
@@ -591,8 +609,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
   __shared__ double s_list[kWarps][2];
   __shared__ GradFactors s_factors;
   extern __shared__ __align__(16) unsigned char s_dyn[];
-  const int part = static_cast<int>(blockIdx.x) % A.parts;
-  const int64_t row = blockIdx.x / A.parts;
+  const int part = cluster_rank();
+  const int64_t row = cluster_id();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Columns<T> C(static_cast<const T *>(A.logits) + row * A.ld, A.V, part, A.span);
   const float w = A.weight ? A.weight[row] : 1.0f;
@@ -794,11 +812,10 @@ size_t distill_smem(DistillArgs &A) {
 }
 
 // CTAs per row.  The loss alone: whole rows while they fill the GPU's CTA
-// slots.  With the gradient: 32 KB of a row each, which with four CTAs per SM
-// stay in shared memory between the two passes; a row of more than 8 x 64 KB
-// is read a second time beyond that.  Either way more CTAs, up to 8, while
-// the rows would leave slots empty, and so many that a CTA's bits of its
-// columns stay within 24 KB.
+// slots.  With the gradient: 32 KB of a row each, of which five CTAs share an
+// SM's shared memory; a row of more than 8 x 64 KB is read a second time
+// beyond that.  Either way more CTAs, up to 8, while the rows would leave
+// slots empty, and so many that a CTA's bits of its columns stay within 24 KB.
 template <typename T, bool REST, bool GRAD>
 cudaError_t launch_distill_as(DistillArgs &A, cudaStream_t st) {
   constexpr int N = RowElem<T>::N;
@@ -812,7 +829,8 @@ cudaError_t launch_distill_as(DistillArgs &A, cudaStream_t st) {
   parts = parts < kMaxCluster ? parts : kMaxCluster;
   A.parts = parts;
   A.span = (vecs + parts - 1) / parts;
-  A.resident = GRAD ? (A.span < kResident / 16 ? A.span : kResident / 16) : 0;
+  const int most = kResident / 16 / kStep * kStep;
+  A.resident = GRAD ? (A.span < most ? A.span : most) : 0;
   if (A.span > kMaxSpan) return cudaErrorInvalidConfiguration;
   const int64_t ctas = static_cast<int64_t>(A.N) * parts;
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
@@ -881,7 +899,9 @@ pz_status distill_args(const char *who, DistillArgs *A, const void *logits, pz_d
   if (t->mode != PZ_DISTILL_LIST && t->mode != PZ_DISTILL_REST) return bad(PZ_ERR_INVALID_ARGS, "bad mode");
   if (!(t->temperature >= 1e-6f && t->temperature <= 1e6f))
     return bad(PZ_ERR_INVALID_ARGS, "temperature outside [1e-6, 1e6]");
-  if (misaligned(logits, elem_bytes(dtype))) return bad(PZ_ERR_INVALID_ARGS, "pointer not aligned to its elements");
+  if (misaligned(logits, elem_bytes(dtype)) || misaligned(t->ids, 4) || misaligned(t->values, 4) ||
+      misaligned(t->n_list, 4) || misaligned(t->weight, 4))
+    return bad(PZ_ERR_INVALID_ARGS, "pointer not aligned to its elements");
   if (t->K > PZ_TOP_K_MAX) return bad(PZ_ERR_UNSUPPORTED, "lists of more than 1024 ids");
   if (V > PZ_DISTILL_MAX_VOCAB) return bad(PZ_ERR_UNSUPPORTED, "more than 2^20 columns");
   A->logits = logits;
@@ -924,8 +944,8 @@ pz_status pz_distill_forward(const void *logits, pz_dtype dtype, int N, int V, i
   pz::DistillArgs A{};
   pz_status s = pz::distill_args("pz_distill_forward", &A, logits, dtype, N, V, ld, target);
   if (s != PZ_OK) return s;
-  if (!loss || pz::misaligned(stats, 16))
-    return pz::report(PZ_ERR_INVALID_ARGS, "pz_distill_forward: no loss, or stats not 16-byte aligned");
+  if (!loss || pz::misaligned(loss, 4) || pz::misaligned(stats, 16))
+    return pz::report(PZ_ERR_INVALID_ARGS, "pz_distill_forward: no loss, or loss or stats (16 bytes) not aligned");
   if (N == 0) return PZ_OK;
   A.loss = loss;
   A.stats = reinterpret_cast<float4 *>(stats);
@@ -940,8 +960,8 @@ pz_status pz_distill_backward(const void *logits, pz_dtype dtype, int N, int V, 
   pz::DistillArgs A{};
   pz_status s = pz::distill_args("pz_distill_backward", &A, logits, dtype, N, V, ld, target);
   if (s != PZ_OK) return s;
-  if (!stats || pz::misaligned(stats, 16))
-    return pz::report(PZ_ERR_INVALID_ARGS, "pz_distill_backward: stats missing or not 16-byte aligned");
+  if (!stats || pz::misaligned(stats, 16) || pz::misaligned(grad_loss, 4))
+    return pz::report(PZ_ERR_INVALID_ARGS, "pz_distill_backward: no stats, or stats (16 bytes) or grad_loss not aligned");
   s = pz::distill_grad_args("pz_distill_backward: grad is the logits' buffer itself (same ld) or apart from it", &A,
                             dtype, grad, ld_grad);
   if (s != PZ_OK || N == 0) return s;
@@ -959,7 +979,8 @@ pz_status pz_distill_loss_grad(const void *logits, pz_dtype dtype, int N, int V,
   pz::DistillArgs A{};
   pz_status s = pz::distill_args("pz_distill_loss_grad", &A, logits, dtype, N, V, ld, target);
   if (s != PZ_OK) return s;
-  if (!loss) return pz::report(PZ_ERR_INVALID_ARGS, "pz_distill_loss_grad: no loss");
+  if (!loss || pz::misaligned(loss, 4))
+    return pz::report(PZ_ERR_INVALID_ARGS, "pz_distill_loss_grad: no loss, or loss not aligned");
   s = pz::distill_grad_args("pz_distill_loss_grad: grad is the logits' buffer itself (same ld) or apart from it", &A,
                             dtype, grad, ld_grad);
   if (s != PZ_OK || N == 0) return s;

@@ -530,6 +530,8 @@ pz_status check_quantize(const void *x, pz_dtype dtype, int rows, int cols, int6
     return report(PZ_ERR_INVALID_ARGS, "pz_quantize_rows_i8: bad dtype");
   if (misaligned(x, elem_bytes(dtype)) || misaligned(q, 16) || ld_q % 16 != 0 || misaligned(scale, 4))
     return report(PZ_ERR_INVALID_ARGS, "pz_quantize_rows_i8: q and its rows start on 16 bytes, x on its elements");
+  if (rows > 0 && overlap(x, rows_bytes(rows, cols, ld, elem_bytes(dtype)), q, rows_bytes(rows, cols, ld_q, 1)))
+    return report(PZ_ERR_INVALID_ARGS, "pz_quantize_rows_i8: q lies over x");
   return PZ_OK;
 }
 
@@ -542,6 +544,11 @@ pz_status check_matmul(const MatmulArgs &A, pz_dtype out_dtype) {
   if (misaligned(A.a, 16) || misaligned(A.w, 16) || A.ld_a % 16 != 0 || A.ld_w % 16 != 0 || misaligned(A.a_scale, 4) ||
       misaligned(A.w_scale, 4) || misaligned(A.out, elem_bytes(out_dtype)))
     return report(PZ_ERR_INVALID_ARGS, "pz_matmul_i8: 8-bit rows start on 16 bytes, out on its elements");
+  if (A.M > 0 && (overlap(A.out, rows_bytes(A.M, A.N, A.ld_out, elem_bytes(out_dtype)), A.w,
+                          rows_bytes(A.N, A.K, A.ld_w, 1)) ||
+                  overlap(A.out, rows_bytes(A.M, A.N, A.ld_out, elem_bytes(out_dtype)), A.a,
+                          rows_bytes(A.M, A.K, A.ld_a, 1))))
+    return report(PZ_ERR_INVALID_ARGS, "pz_matmul_i8: out lies over a or w");
   if (A.K >= PZ_MATMUL_I8_MAX_K)
     return report(PZ_ERR_UNSUPPORTED, "pz_matmul_i8: K of 2^17 or more may overflow the 32-bit sums");
   return PZ_OK;

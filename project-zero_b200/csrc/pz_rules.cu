@@ -13,8 +13,12 @@
 //             object with a key twice is)
 //   mask      v's bit is 0: x = -inf, whatever x was (NaN and inf included)
 //
-// Bound: HBM.  Out of place every logit is read and written once; in place
-// only the vectors that something changes are touched.
+// Bound: HBM.  Out of place every logit is read and written once (1024 rows of
+// 128256 f32: 165 us without rules, 5.3 TB/s of a copy's 6.5; 167 with masks;
+// 199 with 1024 history ids a row, each of which is another 32-byte sector to
+// fetch and to write).  In place only the vectors that something changes are
+// touched: 4096 rows of 151936 bf16 under masks, half of them random, 343 us;
+// a sector that a mask takes part of is read and written whole, 1.65 GB there.
 //
 // A CTA takes a part of a row.  Four warps pass along its columns and know
 // the mask alone.  Two more work out the listed ids meanwhile: those that lie
@@ -496,7 +500,10 @@ extern "C" pz_status pz_process_logits(const void *logits, pz_dtype dtype, int B
                         : (R.mask_rows < (R.mask_index ? 1 : B) || R.mask_ld < (static_cast<int64_t>(V) + 31) / 32))
     return report(PZ_ERR_INVALID_ARGS, "pz_process_logits: mask rows hold ceil(V/32) words, one row per logits row or per index");
   const size_t es = pz::elem_bytes(dtype), eo = pz::elem_bytes(out_dtype);
-  if (pz::misaligned(logits, es) || pz::misaligned(out, eo) || pz::misaligned(R.mask, 4))
+  const void *words[] = {R.cfg, R.hist, R.hist_off, R.bias_ids, R.bias_vals, R.bias_off, R.mask, R.mask_index, n_allowed};
+  bool crooked = pz::misaligned(logits, es) || pz::misaligned(out, eo);
+  for (const void *p : words) crooked |= pz::misaligned(p, 4);
+  if (crooked)
     return report(PZ_ERR_INVALID_ARGS, "pz_process_logits: pointer not aligned to its elements");
   if (B == 0) return PZ_OK;
   const bool inplace = out == logits;

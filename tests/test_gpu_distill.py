@@ -244,6 +244,44 @@ def test_same_bits_each_time_and_in_a_graph(cuda, pz):
     assert all(torch.equal(a, l0) and torch.equal(b, g0) for a, b in outs)
 
 
+def test_autograd_on_streams_and_in_a_graph(cuda, pz):
+    """The differentiable form on a stream that is not the current one's, and
+    forward and backward captured together."""
+    torch = cuda
+    N, V, K = 12, 20003, 10
+    x, ids, t, n, w = make(14, N, V, K, False)
+    ids_d, t_d, n_d, w_d = (torch.from_numpy(a).cuda() for a in (ids, t, n, w))
+    kw = dict(weight=w_d, temperature=2.0, n_list=n_d)
+
+    def both(leaf):
+        loss = pz.distill_loss(leaf, ids_d, t_d, **kw)
+        return loss.detach(), torch.autograd.grad(loss.sum(), leaf)[0]
+
+    leaf = torch.from_numpy(x).cuda().requires_grad_(True)
+    want = both(leaf)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = both(leaf)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    del got
+    static = torch.zeros(N, V, device="cuda").requires_grad_(True)
+    with torch.cuda.stream(side):
+        both(static)  # warm-up, as a user captures
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = both(static)
+    for scale in (1.0, 0.5):
+        with torch.no_grad():
+            static.copy_(leaf.detach() * scale)
+        g.replay()
+        torch.cuda.synchronize()
+        ref = both((leaf.detach() * scale).requires_grad_(True))
+        assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
+
+
 def test_offsets_past_32_bits(cuda, pz):
     torch = cuda
     N, V, K, ld = 3, 5000, 9, (1 << 30) + 8

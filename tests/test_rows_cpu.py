@@ -24,6 +24,9 @@ def process(rules=None, *, logits=P, dtype=0, B=2, V=100, ld=100, out=P * 4, out
     dict(hist=P, hist_off=P), dict(bias_ids=P, bias_off=P), dict(bias_vals=P), dict(mask_index=P),
     dict(mask=P, mask_ld=3, mask_rows=2), dict(mask=P, mask_ld=4, mask_rows=1),
     dict(mask=P, mask_ld=4, mask_rows=0, mask_index=P), dict(mask=P + 2, mask_ld=4, mask_rows=2),
+    dict(mask=P, mask_ld=4, mask_rows=2, mask_index=P + 1), dict(hist=P + 2, hist_off=P, cfg=P),
+    dict(hist=P, hist_off=P + 1, cfg=P), dict(hist=P, hist_off=P, cfg=P + 2),
+    dict(bias_ids=P, bias_off=P, bias_vals=P + 3),
 ], ids=str)
 def test_process_refuses(kw):
     assert process(**kw) == BAD
@@ -50,6 +53,7 @@ def calls(t, *, logits=P, dtype=0, N=2, V=100, ld=100, loss=P, stats=P, grad=P *
 
 
 @pytest.mark.parametrize("kw", [dict(ids=None), dict(values=None), dict(K=0), dict(ld_ids=3), dict(ld_values=3),
+                                dict(ids=P + 2), dict(values=P + 1), dict(n_list=P + 2), dict(weight=P + 2),
                                 dict(mode=2), dict(temperature=0.0), dict(temperature=float("nan")),
                                 dict(temperature=float("inf")), dict(temperature=-1.0)], ids=str)
 def test_distill_refuses_targets(kw):
@@ -66,6 +70,7 @@ def test_distill_refuses_rows(kw):
 def test_distill_refuses_outputs_and_limits():
     assert calls(None) == (BAD, BAD, BAD)
     assert calls(target(), loss=None)[0] == BAD and calls(target(), loss=None)[2] == BAD
+    assert calls(target(), loss=P + 2)[0] == BAD and calls(target(), loss=P + 2)[2] == BAD
     assert calls(target(), stats=None)[1] == BAD and calls(target(), stats=P + 4)[:2] == (BAD, BAD)
     for kw in (dict(grad=None), dict(ld_grad=99), dict(grad=P + 400), dict(grad=P, ld_grad=101), dict(grad=P * 4 + 2)):
         assert calls(target(), **kw)[1:] == (BAD, BAD)
@@ -78,16 +83,16 @@ def test_structures_match_the_header():
     assert ctypes.sizeof(pz.LogitsRules) == 80 and ctypes.sizeof(pz.DistillTarget) == 64
 
 
-def head(hidden=P, dtype=0, B=2, dim=64, ld_h=64, w=P, ld_w=64, ws=P, V=100, out=P, out_dtype=0, ld=100, q=P, ld_q=64,
-         s=P):
+def head(hidden=P, dtype=0, B=2, dim=64, ld_h=64, w=P * 2, ld_w=64, ws=P, V=100, out=P * 3, out_dtype=0, ld=100,
+         q=P * 4, ld_q=64, s=P):
     return L.pz_lm_head_logits_i8(hidden, dtype, B, dim, ld_h, w, ld_w, ws, V, out, out_dtype, ld, q, ld_q, s, None)
 
 
 @pytest.mark.parametrize("kw", [
     dict(hidden=None), dict(w=None), dict(ws=None), dict(out=None), dict(q=None), dict(s=None), dict(B=-1),
     dict(dim=0), dict(V=0), dict(ld_h=63), dict(ld_w=48), dict(ld_w=72), dict(ld_q=72), dict(ld_q=48), dict(ld=99),
-    dict(dtype=2), dict(out_dtype=2), dict(w=P + 8), dict(q=P + 8), dict(hidden=P + 2), dict(out=P + 2),
-    dict(ws=P + 2), dict(s=P + 2),
+    dict(dtype=2), dict(out_dtype=2), dict(w=P * 2 + 8), dict(q=P * 4 + 8), dict(hidden=P + 2), dict(out=P * 3 + 2),
+    dict(ws=P + 2), dict(s=P + 2), dict(q=P + 16), dict(out=P * 2 - 64), dict(out=P * 4 + 48),
 ], ids=str)
 def test_head_refuses(kw):
     assert head(**kw) == BAD
@@ -95,10 +100,10 @@ def test_head_refuses(kw):
 
 
 def test_head_limits_and_empty():
-    big = dict(dim=1 << 17, ld_h=1 << 17, ld_w=1 << 17, ld_q=1 << 17)
+    big = dict(dim=1 << 17, ld_h=1 << 17, ld_w=1 << 17, ld_q=1 << 17, hidden=1 << 30, w=1 << 31, out=1 << 32, q=1 << 33)
     assert head(**big) == UNSUPPORTED
     assert head(B=0) == OK
     assert L.pz_matmul_i8(P, 64, P, 0, P, 64, P, 10, 64, P, 0, 10, None) == OK
-    assert L.pz_matmul_i8(P, 64, None, 2, P, 64, P, 10, 64, P, 0, 10, None) == BAD
+    assert L.pz_matmul_i8(P, 64, None, 2, P * 2, 64, P, 10, 64, P * 3, 0, 10, None) == BAD
     assert L.pz_quantize_rows_i8(P, 0, 0, 64, 64, P, 64, P, None) == OK
     assert L.pz_quantize_rows_i8(P, 0, 2, 64, 64, P, 60, P, None) == BAD
