@@ -275,14 +275,14 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
       const int j = tid + e * kThreads;
       joined[e] = -1.0f;
       if (j < A.K && L.id[j] >= 0) {
-        float all = 0.0f;
+        double all = 0.0;
         bool first = true;
         for (int i = 0; i < A.K; i++)
           if (L.id[i] == L.id[j]) {
             first &= i >= j;
-            all = __fadd_rn(all, L.p[i]);
+            all += L.p[i];
           }
-        if (first) joined[e] = all;
+        if (first) joined[e] = static_cast<float>(all);
       }
     }
     __syncthreads();

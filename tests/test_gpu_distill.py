@@ -114,6 +114,36 @@ def test_rows_longer_than_the_registers_hold(cuda, pz, dtype):
 
 
 @pytest.mark.parametrize("rest", [False, True], ids=["list", "rest"])
+def test_the_longest_rows_and_lists(cuda, pz, rest):
+    torch = cuda
+    N, V, K = 2, 1 << 20, 1024
+    x, ids, t, n, w = make(31, N, V, K, rest, odd=False)
+    for how, inplace in (("one", True), ("both", False)):
+        got = run(torch, pz, x, ids, t, n, w, 1.0, rest, torch.float32, how=how, inplace=inplace)
+        check(x, ids, t, n, w, 1.0, rest, *got, 2.0 ** -24)
+
+
+@pytest.mark.parametrize("rest", [False, True], ids=["list", "rest"])
+@pytest.mark.parametrize("shape", [(9, 5, 12), (6, 40, 300), (4, 3000, 1024)], ids=str)
+def test_ids_listed_many_times(cuda, pz, shape, rest):
+    """Lists longer than the vocabulary, ids that repeat and leave it; the
+    last row lists one id only."""
+    torch = cuda
+    N, V, K = shape
+    r = np.random.default_rng(K)
+    x = (r.standard_normal((N, V)) * 3).astype(np.float32)
+    ids = r.integers(-2, V + 2, (N, K)).astype(np.int32)
+    ids[N - 1] = 1
+    t = r.standard_normal((N, K)).astype(np.float32)
+    if rest:  # the mass of the ids that count stays below one
+        t = (t - np.log(np.exp(t.astype(np.float64)).sum(1, keepdims=True)) - 0.2).astype(np.float32)
+    n, w = np.full(N, K, np.int32), np.ones(N, np.float32)
+    for how in ("one", "both"):
+        got = run(torch, pz, x, ids, t, n, w, 1.0, rest, torch.float32, how=how)
+        check(x, ids, t, n, w, 1.0, rest, *got, 2.0 ** -24)
+
+
+@pytest.mark.parametrize("rest", [False, True], ids=["list", "rest"])
 def test_values_at_the_edges(cuda, pz, rest):
     torch = cuda
     N, V, K = 14, 5000, 8

@@ -76,7 +76,7 @@ SHAPES = [
     # M, N, K
     (1, 1, 1), (1, 130, 33), (2, 127, 128), (3, 129, 16), (15, 300, 100), (16, 128, 256), (17, 1000, 129),
     (33, 500, 640), (64, 257, 1000), (100, 700, 4096), (129, 333, 200), (255, 129, 96), (256, 640, 512),
-    (257, 1001, 300), (300, 19000, 64), (513, 400, 2560), (1, 40000, 512), (8, 32003, 131),
+    (257, 1001, 300), (300, 19000, 64), (64, 257, 40), (65, 1, 16), (70, 255, 1), (513, 3, 131), (1000, 257, 700), (513, 400, 2560), (1, 40000, 512), (8, 32003, 131),
 ]
 
 
