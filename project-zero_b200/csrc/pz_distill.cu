@@ -54,8 +54,6 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;              // 16-byte vectors that a thread works on at a time
 constexpr int kStep = kBatch * kThreads;
 constexpr int kEntries = (PZ_TOP_K_MAX + kThreads - 1) / kThreads;  // most list entries of a thread
-constexpr int kFlagWords = 4;
-constexpr int kMaxSpan = kFlagWords * 32 * kStep;   // vectors of a span: a flag per batch of a thread
 constexpr int kMaxCluster = 8;         // the portable cluster size
 constexpr int kCtasPerSm = 7;
 constexpr int kResident = 64 * 1024;   // most bytes of a row that a CTA keeps in shared memory
@@ -82,6 +80,7 @@ struct DistillArgs {
   int span;   // vectors per CTA
   int bit_words;  // words of a CTA's bits of listed columns, a multiple of 4
   int resident;   // vectors of the span that stay in shared memory
+  int flag_shift; // batches of a thread per flag: 2^flag_shift, so that 32 flags cover the span
 };
 
 // 2^x, fp32 results below 2^-126 flushed to zero (they are lost in any sum
@@ -96,7 +95,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // j % kThreads, which alone reads and writes it once the list is set up.
 struct List {
   uint32_t *bits;  // one bit per column of the CTA's span: listed
-  uint32_t flags[kFlagWords];  // this thread's batches that hold a listed column
+  uint32_t flags;  // REST: this thread's batches (groups of 2^flag_shift) that hold a listed column
   int32_t *id;     // [K]; -1: not in this CTA's columns, ignored, or a later entry of an id listed twice
   float *p;        // [K] probabilities
   float *log_p;    // [K]
@@ -145,7 +144,7 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
   __shared__ int s_seen[kWarps], s_bad[kWarps];
   __shared__ double s_sum[kWarps];
   __shared__ int s_twice, s_gap;
-  __shared__ uint32_t s_flags[REST ? kFlagWords : 1][REST ? kThreads : 1];
+  __shared__ uint32_t s_flags[REST ? kThreads : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int busy = min((A.K + 31) / 32, kWarps);  // warps with an entry
   List L;
@@ -191,10 +190,7 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
   }
   for (int i = tid; i < A.bit_words / 4; i += kThreads) reinterpret_cast<uint4 *>(L.bits)[i] = make_uint4(0u, 0u, 0u, 0u);
   if (tid == 0) s_twice = s_gap = 0;
-  if (REST) {
-#pragma unroll
-    for (int i = 0; i < kFlagWords; i++) s_flags[i][tid] = 0u;
-  }
+  if (REST) s_flags[tid] = 0u;
   __syncthreads();
   top = -INFINITY;
   seen = bad = 0;
@@ -232,8 +228,8 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
         const uint32_t bit = 1u << ((id - sp.c0) & 31);
         L.s[j] = own[e];
         if (REST) {
-          const int vec = (id - sp.c0) / RowElem<T>::N, batch = vec / kStep;
-          atomicOr(&s_flags[batch >> 5][vec % kThreads], 1u << (batch & 31));
+          const int vec = (id - sp.c0) / RowElem<T>::N;
+          atomicOr(&s_flags[vec % kThreads], 1u << (vec / kStep >> A.flag_shift));
         }
         if (atomicOr(&L.bits[(id - sp.c0) >> 5], bit) & bit) s_twice = 1;
       } else {
@@ -245,10 +241,7 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
     if (lane == 0) s_sum[warp] = sum;
   }
   __syncthreads();
-  if (REST) {
-#pragma unroll
-    for (int i = 0; i < kFlagWords; i++) L.flags[i] = s_flags[i][tid];
-  }
+  L.flags = REST ? s_flags[tid] : 0u;
   double sum = 0.0;
   for (int i = 0; i < busy; i++) sum += s_sum[i];
   if (!REST) {
@@ -556,16 +549,11 @@ __device__ __forceinline__ void grad_stream(const Columns<T> &C, const Gradient<
 // One batch into a thread's running maximum and sum (two sums, of the even
 // and the odd columns).  REST: listed ids are left out; few batches hold any.
 template <typename T, bool REST>
-__device__ __forceinline__ void sum_batch(const List &L, const Columns<T> &C, float c, uint4 *raw, int kb, float &m,
-                                          f32x2 &s) {
+__device__ __forceinline__ void sum_batch(const List &L, const Columns<T> &C, float c, int flag_shift, uint4 *raw,
+                                          int kb, float &m, f32x2 &s) {
   constexpr int N = RowElem<T>::N;
   if (REST) {
-    const int batch = (kb - C.sp.k0) / kStep;
-    uint32_t f = L.flags[0];
-#pragma unroll
-    for (int i = 1; i < kFlagWords; i++)
-      if (batch >= 32 * i) f = L.flags[i];
-    if ((f >> (batch & 31)) & 1u) {
+    if ((L.flags >> ((kb - C.sp.k0) / kStep >> flag_shift)) & 1u) {
 #pragma unroll
       for (int i = 0; i < kBatch; i++) {
         const int u = (kb + static_cast<int>(threadIdx.x) + i * kThreads - C.sp.k0) * N;
@@ -650,10 +638,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
     if (GRAD && kb < C.sp.k1) C.load(kb, now);
     for (; kb < C.sp.k1; kb += 2 * kStep) {
       if (kb + kStep < C.sp.k1) C.load(kb + kStep, next);
-      sum_batch<T, REST>(L, C, A.c, now, kb, m, s);
+      sum_batch<T, REST>(L, C, A.c, A.flag_shift, now, kb, m, s);
       if (kb + kStep < C.sp.k1) {
         if (kb + 2 * kStep < C.sp.k1) C.load(kb + 2 * kStep, now);
-        sum_batch<T, REST>(L, C, A.c, next, kb + kStep, m, s);
+        sum_batch<T, REST>(L, C, A.c, A.flag_shift, next, kb + kStep, m, s);
       }
     }
   }
@@ -661,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_kernel(const Dis
     asm volatile("cp.async.wait_all;" ::: "memory");  // a thread reads back what it fetched itself
     for (int kb = C.sp.k0; kb < k_held; kb += kStep) {
       C.held(held, kb, k_held, now);
-      sum_batch<T, REST>(L, C, A.c, now, kb, m, s);
+      sum_batch<T, REST>(L, C, A.c, A.flag_shift, now, kb, m, s);
     }
   }
   MaxSum a{m, 0.0f};
@@ -807,6 +795,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) distill_backward_kernel(
 template <typename T>
 size_t distill_smem(DistillArgs &A) {
   A.bit_words = (A.span * RowElem<T>::N + 127) / 128 * 4;
+  for (A.flag_shift = 0; (A.span - 1) / kStep >> A.flag_shift >= 32;) A.flag_shift++;
   return static_cast<size_t>(A.resident) * 16 +
          sizeof(uint32_t) * (static_cast<size_t>(A.bit_words) + 4 * static_cast<size_t>(A.K));
 }
@@ -831,7 +820,6 @@ cudaError_t launch_distill_as(DistillArgs &A, cudaStream_t st) {
   A.span = (vecs + parts - 1) / parts;
   const int most = kResident / 16 / kStep * kStep;
   A.resident = GRAD ? (A.span < most ? A.span : most) : 0;
-  if (A.span > kMaxSpan) return cudaErrorInvalidConfiguration;
   const int64_t ctas = static_cast<int64_t>(A.N) * parts;
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
   const size_t smem = distill_smem<T>(A);
