@@ -836,11 +836,13 @@ def _distill_function():
         class Distill(torch.autograd.Function):
             @staticmethod
             def forward(ctx, logits, ids, values, weight, temperature, mode, n_list):
-                N = logits.shape[0]
+                N, V, ld, dev, target = _target(logits, ids, values, weight, temperature, mode, n_list)
                 loss = torch.empty(N, dtype=torch.float32, device=logits.device)
                 stats = torch.empty(N, 4, dtype=torch.float32, device=logits.device)
-                distill_forward(logits, ids, values, loss, stats, weight=weight, temperature=temperature, mode=mode,
-                                n_list=n_list)
+                if N:
+                    _call(_lib.pz_distill_forward, "pz_distill_forward", dev, None, logits.data_ptr(),
+                          Sampler._dtype_code(logits), N, V, ld, ctypes.byref(target), loss.data_ptr(),
+                          stats.data_ptr())
                 ctx.save_for_backward(logits, ids, values, weight, n_list, stats)
                 ctx.how = (temperature, mode)
                 return loss
@@ -849,10 +851,13 @@ def _distill_function():
             @torch.autograd.function.once_differentiable
             def backward(ctx, grad_loss):
                 logits, ids, values, weight, n_list, stats = ctx.saved_tensors
-                temperature, mode = ctx.how
-                grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-                distill_backward(logits, ids, values, stats, grad, grad_loss.contiguous(), weight=weight,
-                                 temperature=temperature, mode=mode, n_list=n_list)
+                N, V, ld, dev, target = _target(logits, ids, values, weight, *ctx.how, n_list)
+                grad = torch.empty(N, V, dtype=logits.dtype, device=logits.device)
+                if N:
+                    grad_loss = grad_loss.contiguous()
+                    _call(_lib.pz_distill_backward, "pz_distill_backward", dev, None, logits.data_ptr(),
+                          Sampler._dtype_code(logits), N, V, ld, ctypes.byref(target), stats.data_ptr(),
+                          grad_loss.data_ptr(), grad.data_ptr(), V)
                 return grad, None, None, None, None, None, None
 
         _distill_fn = Distill
