@@ -24,11 +24,12 @@
 // rho / r hold when the student leaves them next to nothing.  The sum over
 // the list, whose terms nearly cancel against log S, is in fp64.
 //
-// Bound: HBM, and for bf16 loss and gradient together the SMs' issue slots
-// (two exponentials per id and what every warp repeats per row).
+// Bound: HBM; loss and gradient together also by what has to follow one
+// another within a row (fetch, exchange, store), which five CTAs on an SM do
+// not hide altogether.
 //   loss      a row per CTA while the rows fill the GPU, parts of one in a
 //             cluster otherwise; the next batch of vectors in flight while one
-//             is summed.  1024 rows of 128256 f32: 77 us, 6.8 TB/s.
+//             is summed.  1024 rows of 128256 f32: 74 us, 7.1 TB/s.
 //   gradient  from saved statistics: parts of 64 KB, independent CTAs.  2048
 //             rows of 151936 bf16: 190 us, 6.5 TB/s (after a loss of 99 us).
 //   both      one read and one write: a row stays on chip between its two
@@ -800,21 +801,31 @@ size_t distill_smem(DistillArgs &A) {
          sizeof(uint32_t) * (static_cast<size_t>(A.bit_words) + 4 * static_cast<size_t>(A.K));
 }
 
-// CTAs per row.  The loss alone: whole rows while they fill the GPU's CTA
-// slots.  With the gradient: 32 KB of a row each, of which five CTAs share an
-// SM's shared memory; a row of more than 8 x 64 KB is read a second time
-// beyond that.  Either way more CTAs, up to 8, while the rows would leave
-// slots empty, and so many that a CTA's bits of its columns stay within 24 KB.
+// CTAs per row, up to 8.  The loss alone: as many as fill one wave of the
+// GPU's CTA slots (512 rows of 128256 f32: 42.4 us with two, 49.3 with three,
+// 1.5 waves of them); one from there on, two where that leaves the second or
+// third wave less than half full (1100 rows: 111 and 101 us; 2048: 155 and
+// 160).  With the gradient: 32 KB of a row each, of which five CTAs share an
+// SM's shared memory, more while the rows would leave slots empty; a row of
+// more than 8 x 64 KB is read a second time beyond that.  Either way so many
+// that a CTA's bits of its columns stay within 24 KB.
 template <typename T, bool REST, bool GRAD>
 cudaError_t launch_distill_as(DistillArgs &A, cudaStream_t st) {
   constexpr int N = RowElem<T>::N;
   const int vecs = (A.V + 2 * N - 2) / N;  // of a row with the largest shift
-  int parts = GRAD ? (vecs + 2047) / 2048 : 1;
-  const int bits = (A.V + 24 * 1024 * 8 - 1) / (24 * 1024 * 8);
-  parts = parts > bits ? parts : bits;
-  while (parts < kMaxCluster && static_cast<int64_t>(A.N) * parts < kCtasPerSm * current_sms() &&
-         vecs > parts * kBatch * kThreads)
-    parts++;
+  const int slots = kCtasPerSm * current_sms(), wave = slots / A.N;
+  const int least = (A.V + 24 * 1024 * 8 - 1) / (24 * 1024 * 8);  // by the bits
+  const int batches = vecs / kStep;
+  int parts;
+  if (GRAD) {
+    parts = (vecs + 2047) / 2048;
+    if (parts < wave) parts = wave < batches ? wave : batches;
+  } else {
+    const int last = A.N % slots;
+    parts = wave > 0 ? wave : A.N < 3 * slots && last > 0 && last < slots / 2 ? 2 : 1;
+    parts = parts < batches ? parts : batches;
+  }
+  parts = parts > least ? parts : least;  // (at least one)
   parts = parts < kMaxCluster ? parts : kMaxCluster;
   A.parts = parts;
   A.span = (vecs + parts - 1) / parts;
@@ -856,7 +867,8 @@ cudaError_t launch_backward(DistillArgs &A, cudaStream_t st) {
   constexpr int N = RowElem<T>::N;
   const int vecs = (A.V + 2 * N - 2) / N;
   A.parts = (vecs + 4095) / 4096;
-  while (static_cast<int64_t>(A.N) * A.parts < kCtasPerSm * current_sms() && vecs > A.parts * kThreads) A.parts *= 2;
+  const int wave = kCtasPerSm * current_sms() / A.N, most = vecs / kThreads;
+  if (A.parts < wave && A.parts < most) A.parts = wave < most ? wave : most;
   A.span = (vecs + A.parts - 1) / A.parts;
   const int64_t ctas = static_cast<int64_t>(A.N) * A.parts;
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
