@@ -643,29 +643,46 @@ def configs_to_device(cfg_np, device="cuda"):
 # --------------------------------------------------------------------------
 # Rows of logits outside the sampler: constraints, distillation.
 # --------------------------------------------------------------------------
-# (these run at every call of a decode step: indexes instead of device objects,
-# and the raw stream where torch hands it out)
-_raw_stream = None
+# (these run at every call of a decode step: torch looked up once, indexes
+# instead of device objects, and torch's raw calls where it hands them out)
+class _Torch:
+    """torch, its current device and raw current stream, and dtype codes; made
+    at the first call, so that importing this module does not import torch."""
 
-
-def _current_raw_stream(dev):
-    global _raw_stream
-    if _raw_stream is None:
+    def __init__(self):
         import torch
-        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        self.f32, self.i32, self.i8 = torch.float32, torch.int32, torch.int8
+        self.words = (torch.int32, torch.uint32)
+        self.codes = {torch.float32: PZ_DTYPE_F32, torch.bfloat16: PZ_DTYPE_BF16}
+        self.device = torch.cuda.device
+        self.current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda d: torch.cuda.current_stream(d).cuda_stream)
-    return _raw_stream(dev)
+
+
+_T = None
+
+
+def _torch():
+    global _T
+    _T = _Torch()
+    return _T
+
+
+def _code(T, t):
+    code = T.codes.get(t.dtype)
+    return Sampler._dtype_code(t) if code is None else code  # (which raises)
 
 
 def _call(fn, name, dev, stream, *args):
     """Calls a context-free entry on device `dev`, on `stream` or that
     device's current stream."""
-    import torch
-    handle = _current_raw_stream(dev) if stream is None else _stream_handle(stream)
-    if dev == torch.cuda.current_device():
+    T = _T
+    handle = T.raw_stream(dev) if stream is None else _stream_handle(stream)
+    if dev == T.current_device():
         st = fn(*args, handle)
     else:
-        with torch.cuda.device(dev):
+        with T.device(dev):
             st = fn(*args, handle)
     if st != PZ_OK:
         raise PZError(st, name)
@@ -708,8 +725,8 @@ def process_logits(logits, out=None, *, cfg=None, hist=None, hist_off=None, bias
     applied to logits [B, V].  out=None works in place; out may be float32
     where the logits are bfloat16.  n_allowed: [B] int32, the ids each row's
     mask leaves.  Returns out."""
-    import torch
-    i32 = torch.int32
+    T = _T or _torch()
+    i32 = T.i32
     B, V, ld = _rows(logits, "logits")
     dev = logits.get_device()
     if out is None:
@@ -729,11 +746,11 @@ def process_logits(logits, out=None, *, cfg=None, hist=None, hist_off=None, bias
             rules.cfg = cfg.data_ptr()
     if bias_ids is not None and bias_ids.numel():
         rules.bias_ids = _vector(bias_ids, "bias_ids", 0, i32, dev)
-        rules.bias_vals = _vector(bias_vals, "bias_vals", bias_ids.numel(), torch.float32, dev)
+        rules.bias_vals = _vector(bias_vals, "bias_vals", bias_ids.numel(), T.f32, dev)
         rules.bias_off = _vector(bias_off, "bias_off", B + 1, i32, dev)
     if mask is not None:
         rows, words, mask_ld = _rows(mask, "mask")
-        if mask.dtype not in (i32, torch.uint32) or mask.get_device() != dev:
+        if mask.dtype not in T.words or mask.get_device() != dev:
             raise ValueError("mask has to be int32 or uint32 words on the logits' device")
         if words * 32 < V:
             raise ValueError(f"mask rows of {words} words do not cover {V} ids")
@@ -744,28 +761,28 @@ def process_logits(logits, out=None, *, cfg=None, hist=None, hist_off=None, bias
     n_out = _vector(n_allowed, "n_allowed", B, i32, dev)
     if B == 0:
         return out
-    _call(_lib.pz_process_logits, "pz_process_logits", dev, stream, logits.data_ptr(), Sampler._dtype_code(logits),
-          B, V, ld, ctypes.byref(rules), out.data_ptr(), Sampler._dtype_code(out), ld_out, n_out)
+    _call(_lib.pz_process_logits, "pz_process_logits", dev, stream, logits.data_ptr(), _code(T, logits),
+          B, V, ld, ctypes.byref(rules), out.data_ptr(), _code(T, out), ld_out, n_out)
     return out
 
 
 def _target(logits, ids, values, weight, temperature, mode, n_list):
     """The checked arguments that the distillation calls share: rows, columns,
     row stride and device of the logits, and the target."""
-    import torch
+    T = _T or _torch()
     N, V, ld = _rows(logits, "logits")
     dev = logits.get_device()
     rows, K, ld_ids = _rows(ids, "ids")
     _, _, ld_values = _rows(values, "values", ids)
-    if ids.dtype is not torch.int32 or values.dtype is not torch.float32:
+    if ids.dtype is not T.i32 or values.dtype is not T.f32:
         raise TypeError("ids have to be int32 and values float32")
     if rows != N or ids.get_device() != dev:
         raise ValueError("ids and values have to be [rows of the logits, K] on the logits' device")
     if V == 0:
         raise ValueError("logits without columns")
     return N, V, ld, dev, DistillTarget(ids.data_ptr(), values.data_ptr(), ld_ids, ld_values, K, mode,
-                                        _vector(n_list, "n_list", N, torch.int32, dev),
-                                        _vector(weight, "weight", N, torch.float32, dev), temperature, 0)
+                                        _vector(n_list, "n_list", N, T.i32, dev),
+                                        _vector(weight, "weight", N, T.f32, dev), temperature, 0)
 
 
 def _gradient(logits, grad):
@@ -781,12 +798,12 @@ def distill_forward(logits, ids, values, loss, stats=None, *, weight=None, tempe
     against the teacher's lists ids [N, K] int32 / values [N, K] float32
     (mode DISTILL_LIST or DISTILL_REST), and, for distill_backward, stats
     [N, 4] float32.  Returns loss."""
-    import torch
+    T = _T or _torch()
     N, V, ld, dev, target = _target(logits, ids, values, weight, temperature, mode, n_list)
-    out = _vector(loss, "loss", N, torch.float32, dev), _vector(stats, "stats", 4 * N, torch.float32, dev)
+    out = _vector(loss, "loss", N, T.f32, dev), _vector(stats, "stats", 4 * N, T.f32, dev)
     if N == 0:
         return loss
-    _call(_lib.pz_distill_forward, "pz_distill_forward", dev, stream, logits.data_ptr(), Sampler._dtype_code(logits),
+    _call(_lib.pz_distill_forward, "pz_distill_forward", dev, stream, logits.data_ptr(), _code(T, logits),
           N, V, ld, ctypes.byref(target), *out)
     return loss
 
@@ -796,14 +813,14 @@ def distill_backward(logits, ids, values, stats, grad, grad_loss=None, *, weight
     """pz_distill_backward: grad [N, V] (the logits' type; may be the logits
     themselves) of sum(grad_loss * loss) from distill_forward's stats on the
     same arguments.  Returns grad."""
-    import torch
+    T = _T or _torch()
     N, V, ld, dev, target = _target(logits, ids, values, weight, temperature, mode, n_list)
     ld_grad = _gradient(logits, grad)
-    given = _vector(stats, "stats", 4 * N, torch.float32, dev), _vector(grad_loss, "grad_loss", N, torch.float32, dev)
+    given = _vector(stats, "stats", 4 * N, T.f32, dev), _vector(grad_loss, "grad_loss", N, T.f32, dev)
     if N == 0:
         return grad
     _call(_lib.pz_distill_backward, "pz_distill_backward", dev, stream, logits.data_ptr(),
-          Sampler._dtype_code(logits), N, V, ld, ctypes.byref(target), *given, grad.data_ptr(), ld_grad)
+          _code(T, logits), N, V, ld, ctypes.byref(target), *given, grad.data_ptr(), ld_grad)
     return grad
 
 
@@ -812,14 +829,14 @@ def distill_loss_grad(logits, ids, values, loss, grad, *, weight=None, temperatu
     """pz_distill_loss_grad: loss [N] and the gradient of its sum, in one
     pass over the logits (grad may be the logits themselves).  Returns
     (loss, grad)."""
-    import torch
+    T = _T or _torch()
     N, V, ld, dev, target = _target(logits, ids, values, weight, temperature, mode, n_list)
     ld_grad = _gradient(logits, grad)
-    out = _vector(loss, "loss", N, torch.float32, dev)
+    out = _vector(loss, "loss", N, T.f32, dev)
     if N == 0:
         return loss, grad
     _call(_lib.pz_distill_loss_grad, "pz_distill_loss_grad", dev, stream, logits.data_ptr(),
-          Sampler._dtype_code(logits), N, V, ld, ctypes.byref(target), out, grad.data_ptr(), ld_grad)
+          _code(T, logits), N, V, ld, ctypes.byref(target), out, grad.data_ptr(), ld_grad)
     return loss, grad
 
 
@@ -832,16 +849,17 @@ def _distill_function():
     global _distill_fn
     if _distill_fn is None:
         import torch
+        T = _T or _torch()
 
         class Distill(torch.autograd.Function):
             @staticmethod
             def forward(ctx, logits, ids, values, weight, temperature, mode, n_list):
                 N, V, ld, dev, target = _target(logits, ids, values, weight, temperature, mode, n_list)
-                loss = torch.empty(N, dtype=torch.float32, device=logits.device)
-                stats = torch.empty(N, 4, dtype=torch.float32, device=logits.device)
+                loss = torch.empty(N, dtype=T.f32, device=logits.device)
+                stats = torch.empty(N, 4, dtype=T.f32, device=logits.device)
                 if N:
                     _call(_lib.pz_distill_forward, "pz_distill_forward", dev, None, logits.data_ptr(),
-                          Sampler._dtype_code(logits), N, V, ld, ctypes.byref(target), loss.data_ptr(),
+                          _code(T, logits), N, V, ld, ctypes.byref(target), loss.data_ptr(),
                           stats.data_ptr())
                 ctx.save_for_backward(logits, ids, values, weight, n_list, stats)
                 ctx.how = (temperature, mode)
@@ -856,7 +874,7 @@ def _distill_function():
                 if N:
                     grad_loss = grad_loss.contiguous()
                     _call(_lib.pz_distill_backward, "pz_distill_backward", dev, None, logits.data_ptr(),
-                          Sampler._dtype_code(logits), N, V, ld, ctypes.byref(target), stats.data_ptr(),
+                          _code(T, logits), N, V, ld, ctypes.byref(target), stats.data_ptr(),
                           grad_loss.data_ptr(), grad.data_ptr(), V)
                 return grad, None, None, None, None, None, None
 
@@ -877,9 +895,8 @@ def distill_loss(logits, ids, values, *, weight=None, temperature=1.0, mode=DIST
 def _i8(t, name, dev, rows, cols):
     """Checks an int8 [rows, cols] tensor; its row stride (of a single row
     any: the library wants a multiple of 16)."""
-    import torch
     r, c, ld = _rows(t, name)
-    if t.dtype is not torch.int8 or r != rows or c != cols or t.get_device() != dev:
+    if t.dtype is not _T.i8 or r != rows or c != cols or t.get_device() != dev:
         raise ValueError(f"{name} has to be int8 [{rows}, {cols}] on the same device")
     return (c + 15) // 16 * 16 if r <= 1 else ld
 
@@ -889,14 +906,14 @@ def quantize_rows_i8(x, q, scale, stream=None):
     cols] int8 (rows a multiple of 16 bytes apart, e.g. torch.empty(rows,
     (cols + 15) // 16 * 16, dtype=torch.int8)[:, :cols]) and scale [rows]
     float32.  Returns (q, scale)."""
-    import torch
+    T = _T or _torch()
     rows, cols, ld = _rows(x, "x")
     dev = x.get_device()
     ld_q = _i8(q, "q", dev, rows, cols)
-    out = _vector(scale, "scale", rows, torch.float32, dev)
+    out = _vector(scale, "scale", rows, T.f32, dev)
     if rows == 0:
         return q, scale
-    _call(_lib.pz_quantize_rows_i8, "pz_quantize_rows_i8", dev, stream, x.data_ptr(), Sampler._dtype_code(x), rows,
+    _call(_lib.pz_quantize_rows_i8, "pz_quantize_rows_i8", dev, stream, x.data_ptr(), _code(T, x), rows,
           cols, ld, q.data_ptr(), ld_q, out)
     return q, scale
 
@@ -904,16 +921,16 @@ def quantize_rows_i8(x, q, scale, stream=None):
 def matmul_i8(a, a_scale, w, w_scale, out, stream=None):
     """pz_matmul_i8: out [M, N] (float32 or bfloat16) = (a [M, K] @ w [N, K]^T)
     * a_scale [M] * w_scale [N], the sums in 32-bit integers.  Returns out."""
-    import torch
+    T = _T or _torch()
     M, N, ld = _rows(out, "out")
     dev = out.get_device()
     K = a.shape[-1]
     ld_a, ld_w = _i8(a, "a", dev, M, K), _i8(w, "w", dev, N, K)
-    scales = (_vector(a_scale, "a_scale", M, torch.float32, dev), _vector(w_scale, "w_scale", N, torch.float32, dev))
+    scales = (_vector(a_scale, "a_scale", M, T.f32, dev), _vector(w_scale, "w_scale", N, T.f32, dev))
     if M == 0:
         return out
     _call(_lib.pz_matmul_i8, "pz_matmul_i8", dev, stream, a.data_ptr(), ld_a, scales[0], M, w.data_ptr(), ld_w,
-          scales[1], N, K, out.data_ptr(), Sampler._dtype_code(out), ld)
+          scales[1], N, K, out.data_ptr(), _code(T, out), ld)
     return out
 
 
@@ -922,18 +939,18 @@ def lm_head_i8(hidden, w_q, w_scale, logits, hidden_q, hidden_scale, stream=None
     [B, dim] (float32 or bfloat16), quantised per row into hidden_q [B, dim]
     int8 / hidden_scale [B], times the classifier w_q [V, dim] int8 with
     w_scale [V] (quantize_rows_i8).  Returns logits."""
-    import torch
+    T = _T or _torch()
     B, dim, ld_hidden = _rows(hidden, "hidden")
     rows, V, ld = _rows(logits, "logits")
     dev = hidden.get_device()
     if rows != B or logits.get_device() != dev:
         raise ValueError("logits have to be [B, V] on the hidden rows' device")
     ld_w, ld_q = _i8(w_q, "w_q", dev, V, dim), _i8(hidden_q, "hidden_q", dev, B, dim)
-    scales = (_vector(w_scale, "w_scale", V, torch.float32, dev),
-              _vector(hidden_scale, "hidden_scale", B, torch.float32, dev))
+    scales = (_vector(w_scale, "w_scale", V, T.f32, dev),
+              _vector(hidden_scale, "hidden_scale", B, T.f32, dev))
     if B == 0:
         return logits
     _call(_lib.pz_lm_head_logits_i8, "pz_lm_head_logits_i8", dev, stream, hidden.data_ptr(),
-          Sampler._dtype_code(hidden), B, dim, ld_hidden, w_q.data_ptr(), ld_w, scales[0], V, logits.data_ptr(),
-          Sampler._dtype_code(logits), ld, hidden_q.data_ptr(), ld_q, scales[1])
+          _code(T, hidden), B, dim, ld_hidden, w_q.data_ptr(), ld_w, scales[0], V, logits.data_ptr(),
+          _code(T, logits), ld, hidden_q.data_ptr(), ld_q, scales[1])
     return logits
