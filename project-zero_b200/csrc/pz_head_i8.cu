@@ -363,6 +363,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int m0 = tile % A.tok_tiles * A.nt;
       T *out = static_cast<T *>(A.out) + static_cast<int64_t>(m0) * A.ld_out + n;
       const int tokens = min(A.nt, A.M - m0);
+      // the scales are on their way while the sums are waited for
+      const float sw = n < A.N ? A.w_scale[n] : 0.0f;
+      float sa = first + lane < tokens ? __ldcg(A.a_scale + m0 + first + lane) : 0.0f;
       if (ok) ok = mbar_wait(sum + 8 * acc, (t >> 1) & 1, &s_stop);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) {
@@ -371,11 +374,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         continue;
       }
       tc_fence_after();
-      const float sw = n < A.N ? A.w_scale[n] : 0.0f;
       const uint32_t at = tmem + static_cast<uint32_t>(acc * (A.cols / 2)) + (static_cast<uint32_t>(quarter * 32) << 16);
       // 32 tokens at a time; each lane fetches one token's scale, ahead of
       // the stores that the compiler may not move a load across
-      float sa = first + lane < tokens ? __ldcg(A.a_scale + m0 + first + lane) : 0.0f;
       constexpr int STEP = 8 * kTcWarps;
       for (int c = first; c < tokens; c += STEP) {
         int v[32];
