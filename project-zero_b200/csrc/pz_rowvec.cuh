@@ -202,21 +202,4 @@ __device__ __forceinline__ uint4 load_row_vec(const T *row, int shift, int V, in
   return RowElem<T>::pack(x);
 }
 
-// Columns [c, c + N) of the output row, those inside [0, V).  `aligned`:
-// whether a whole vector's address is a multiple of 16 bytes.  N is the
-// input vector's length; the output element may be wider (two stores).
-template <int N, typename T>
-__device__ __forceinline__ void store_row_vec(T *row, int V, int c, const float *x, bool aligned) {
-  constexpr int M = RowElem<T>::N;
-  static_assert(N % M == 0, "an output vector is a whole number of 16-byte stores");
-  if (aligned && c >= 0 && c + N <= V) {
-#pragma unroll
-    for (int i = 0; i < N / M; i++) store16(row + c + i * M, RowElem<T>::pack(x + i * M));
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < N; j++)
-    if (c + j >= 0 && c + j < V) RowElem<T>::put(row + c + j, x[j]);
-}
-
 }  // namespace pz
