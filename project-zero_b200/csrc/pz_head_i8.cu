@@ -24,7 +24,6 @@
 namespace pz {
 namespace {
 
-constexpr int kQuantThreads = 256;
 constexpr int kQuantRes = 4;  // 16-byte vectors of a row that a thread keeps in registers
 
 struct QuantArgs {
@@ -36,68 +35,67 @@ struct QuantArgs {
   float *scale;
 };
 
-// One CTA per row; the row is read once while it fits the registers
-// (16 KB), else a second time from L2.
-template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const QuantArgs A) {
+// One CTA per row; the row is read once while it fits the registers (64 bytes
+// a thread), what is beyond that a second time from L2.  Bound: HBM for rows
+// that fit (128256 x 4096 bf16: 235 us, 6.7 TB/s).  To keep the arithmetic under it:
+// the maximum of magnitudes carries NaN by itself, and adding 1.5 * 2^23
+// rounds to a whole number (to even, as rint does) whose low byte is q.  The
+// product and the sum are separate instructions for one value: the packed
+// forms for two were joined into one, whose single rounding moves ties
+// (63.4999998 became 63 where the rounded product 63.5 gives 64).
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) quantize_kernel(const QuantArgs A) {
   constexpr int N = RowElem<T>::N;
-  constexpr int NT = kQuantThreads;
   pdl_launch_dependents();  // the product may start fetching its weights
   __shared__ float s_top[NT / 32];
-  __shared__ int s_bad[NT / 32];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const T *x_row = static_cast<const T *>(A.x) + row * A.ld;
   int8_t *q_row = A.q + row * A.ld_q;
   const int shift = row_shift(x_row);
   const int vecs = (A.cols + shift + N - 1) / N;
-  uint4 raw[kQuantRes];
-  float top = 0.0f;
-  int bad = 0;
-  auto look = [&](const uint4 &r, int k) {
-    float x[N];
-    RowElem<T>::unpack(r, x);
-    const int c = k * N - shift;
-#pragma unroll
-    for (int j = 0; j < N; j++)
-      if (c + j >= 0 && c + j < A.cols) {
-        bad |= !(fabsf(x[j]) <= 3.402823466e38f);
-        top = fmaxf(top, fabsf(x[j]));
-      }
+  const WholeVecs whole = whole_vecs<T>(shift, A.cols);
+  // columns outside the row as 0: they change no maximum
+  auto is_whole = [&](int k) { return k >= whole.first && k < whole.last; };
+  auto load = [&](int k) {
+    return is_whole(k) ? load16(x_row + (k * N - shift)) : load_edge(x_row, A.cols, k * N - shift, 0.0f);
   };
+  uint4 raw[kQuantRes];
 #pragma unroll
-  for (int i = 0; i < kQuantRes; i++)
-    if (tid + i * NT < vecs) raw[i] = load_row_vec(x_row, shift, A.cols, tid + i * NT);
-#pragma unroll
-  for (int i = 0; i < kQuantRes; i++)
-    if (tid + i * NT < vecs) look(raw[i], tid + i * NT);
-  for (int k = tid + kQuantRes * NT; k < vecs; k += NT) look(load_row_vec(x_row, shift, A.cols, k), k);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  bad = __any_sync(0xFFFFFFFFu, bad);
-  if ((tid & 31) == 0) {
-    s_top[tid >> 5] = top;
-    s_bad[tid >> 5] = bad;
+  for (int i = 0; i < kQuantRes; i++) {
+    const int k = tid + i * NT;
+    raw[i] = is_whole(k) ? load16(x_row + (k * N - shift)) : make_uint4(0u, 0u, 0u, 0u);
   }
+  // the edges once every whole vector is on its way: a call between them would hold them up
+#pragma unroll
+  for (int i = 0; i < kQuantRes; i++)
+    if (tid + i * NT < vecs && !is_whole(tid + i * NT)) raw[i] = load(tid + i * NT);
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kQuantRes; i++) top = max_nan(top, RowElem<T>::max_abs_nan(raw[i]));
+  for (int k = tid + kQuantRes * NT; k < vecs; k += NT) top = max_nan(top, RowElem<T>::max_abs_nan(load(k)));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  if ((tid & 31) == 0) s_top[tid >> 5] = top;
   __syncthreads();
-  for (int i = 0; i < NT / 32; i++) {
-    top = fmaxf(top, s_top[i]);
-    bad |= s_bad[i];
-  }
+  for (int i = 0; i < NT / 32; i++) top = max_nan(top, s_top[i]);
+  const bool bad = !(top <= 3.402823466e38f);  // an infinity or NaN
   const bool some = !bad && top >= 7.888609052e-31f;  // 2^-100
   const float inv = some ? __fdiv_rn(127.0f, top) : 0.0f;
   if (tid == 0) A.scale[row] = bad ? __int_as_float(0x7FC00000) : some ? __fdiv_rn(top, 127.0f) : 0.0f;
-  auto write = [&](const uint4 &r, int k) {
+  auto write = [&](uint4 r, int k) {
+    if (!some) r = make_uint4(0u, 0u, 0u, 0u);  // (inf times 0 is no number)
     float x[N];
     RowElem<T>::unpack(r, x);
-    const int c = k * N - shift;
+    auto whole_number = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.0f)); };
     uint32_t w[N / 4];
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-      const int q = some ? __float2int_rn(__fmul_rn(x[j], inv)) : 0;
-      const uint32_t b = static_cast<uint32_t>(q & 0xFF) << (8 * (j & 3));
-      w[j / 4] = (j & 3) == 0 ? b : (w[j / 4] | b);
+    for (int j = 0; j < N / 4; j++) {
+      const uint32_t lo = __byte_perm(whole_number(x[4 * j]), whole_number(x[4 * j + 1]), 0x0040);
+      const uint32_t hi = __byte_perm(whole_number(x[4 * j + 2]), whole_number(x[4 * j + 3]), 0x0040);
+      w[j] = __byte_perm(lo, hi, 0x5410);
     }
+    const int c = k * N - shift;
     if (shift == 0 && c + N <= A.cols) {
       if constexpr (N == 4)
         *reinterpret_cast<uint32_t *>(q_row + c) = w[0];
@@ -112,14 +110,28 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const QuantArgs
 #pragma unroll
   for (int i = 0; i < kQuantRes; i++)
     if (tid + i * NT < vecs) write(raw[i], tid + i * NT);
-  for (int k = tid + kQuantRes * NT; k < vecs; k += NT) write(load_row_vec(x_row, shift, A.cols, k), k);
+  for (int k = tid + kQuantRes * NT; k < vecs; k += NT) write(load(k), k);
+}
+
+// 128 threads while their registers hold the row (8 KB), 256 beyond.  Both
+// sides, 128 and 256 threads, us: 128256 x 4096 bf16 235 and 357, 32000 x 1000
+// bf16 36 and 66, 1024 x 4096 bf16 3.3 and 4.3; 128256 x 8192 bf16 666 and 489,
+// 512 x 4096 f32 4.1 and 3.0, 1 x 4096 f32 3.3 and 2.0.  Threads in a number
+// set at run time to fit each row were slower than the better of the two.
+template <typename T>
+void launch_quantize_as(const QuantArgs &A, cudaStream_t st) {
+  constexpr int narrow_cols = 128 * kQuantRes * RowElem<T>::N;
+  if (A.cols <= narrow_cols)
+    quantize_kernel<T, 128><<<A.rows, 128, 0, st>>>(A);
+  else
+    quantize_kernel<T, 256><<<A.rows, 256, 0, st>>>(A);
 }
 
 cudaError_t launch_quantize(const QuantArgs &A, pz_dtype dtype, cudaStream_t st) {
   if (dtype == PZ_DTYPE_F32)
-    quantize_kernel<float><<<A.rows, kQuantThreads, 0, st>>>(A);
+    launch_quantize_as<float>(A, st);
   else
-    quantize_kernel<bf16_t><<<A.rows, kQuantThreads, 0, st>>>(A);
+    launch_quantize_as<bf16_t>(A, st);
   return cudaGetLastError();
 }
 

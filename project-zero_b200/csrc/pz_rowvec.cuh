@@ -9,12 +9,14 @@
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 namespace pz {
 
 // Two fp32 values in one 64-bit register: sm_100 adds and multiplies both in
-// one instruction, each rounded as on its own.
+// one instruction.  A product that feeds a sum may be joined with it into one
+// rounding: where two roundings are the definition, take scalars.
 using f32x2 = unsigned long long;
 __device__ __forceinline__ f32x2 pair(float lo, float hi) {
   f32x2 r;
@@ -32,6 +34,13 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
 __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   f32x2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// The larger of two values, NaN where either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
@@ -68,6 +77,11 @@ struct RowElem<float> {
   }
   static __device__ __forceinline__ float max(const uint4 &u) {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+  // the largest magnitude, NaN where any value is
+  static __device__ __forceinline__ float max_abs_nan(const uint4 &u) {
+    return max_nan(max_nan(fabsf(__uint_as_float(u.x)), fabsf(__uint_as_float(u.y))),
+                   max_nan(fabsf(__uint_as_float(u.z)), fabsf(__uint_as_float(u.w))));
   }
   // the elements whose bit is set, -inf for the others
   static __device__ __forceinline__ uint4 keep(const uint4 &u, uint32_t bits) {
@@ -123,6 +137,12 @@ struct RowElem<bf16_t> {
     const __nv_bfloat162 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
     return fmaxf(__low2float(m), __high2float(m));
   }
+  static __device__ __forceinline__ float max_abs_nan(const uint4 &u) {
+    const __nv_bfloat162 *v = reinterpret_cast<const __nv_bfloat162 *>(&u);
+    const __nv_bfloat162 m =
+        __hmax2_nan(__hmax2_nan(__habs2(v[0]), __habs2(v[1])), __hmax2_nan(__habs2(v[2]), __habs2(v[3])));
+    return max_nan(__low2float(m), __high2float(m));
+  }
   // Selectors of a byte permutation for four elements: 0x54 and 0x76 take the
   // two bytes of an element from the second operand, 0x10 and 0x32 (0x44
   // less) from the first.  The product spreads four bits over four bytes.
@@ -167,15 +187,15 @@ __device__ __forceinline__ WholeVecs whole_vecs(int shift, int V) {
   return WholeVecs{shift > 0 ? 1 : 0, (V + shift) / RowElem<T>::N};
 }
 
-// Columns [c, c + N) that reach outside the row, those outside as -inf.  Out
+// Columns [c, c + N) that reach outside the row, those outside as `fill`.  Out
 // of line: at most two vectors of a row take this way.
 template <typename T>
-__device__ __noinline__ uint4 load_edge(const T *row, int V, int c) {
+__device__ __noinline__ uint4 load_edge(const T *row, int V, int c, float fill = -INFINITY) {
   constexpr int N = RowElem<T>::N;
   float x[N];
 #pragma unroll
   for (int j = 0; j < N; j++)
-    x[j] = (c + j >= 0 && c + j < V) ? RowElem<T>::get(row + c + j) : __int_as_float(0xFF800000);
+    x[j] = (c + j >= 0 && c + j < V) ? RowElem<T>::get(row + c + j) : fill;
   return RowElem<T>::pack(x);
 }
 // A packed vector to the columns [c, c + N) of a row, those inside [0, V).
@@ -187,19 +207,6 @@ __device__ __noinline__ void store_edge(T *row, int V, int c, uint4 v) {
 #pragma unroll
   for (int j = 0; j < N; j++)
     if (c + j >= 0 && c + j < V) RowElem<T>::put(row + c + j, x[j]);
-}
-
-// Vector k of the row: packed, columns outside [0, V) as -inf.
-template <typename T>
-__device__ __forceinline__ uint4 load_row_vec(const T *row, int shift, int V, int k) {
-  constexpr int N = RowElem<T>::N;
-  const int c = k * N - shift;
-  if (c >= 0 && c + N <= V) return load16(row + c);
-  float x[N];
-#pragma unroll
-  for (int j = 0; j < N; j++)
-    x[j] = (c + j >= 0 && c + j < V) ? RowElem<T>::get(row + c + j) : __int_as_float(0xFF800000);
-  return RowElem<T>::pack(x);
 }
 
 }  // namespace pz
