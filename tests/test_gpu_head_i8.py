@@ -72,6 +72,51 @@ def test_rows_are_quantised(cuda, pz, shape, dtype):
     assert bool((buf[:rows, cols:] == 99).all()) and bool((buf[rows] == 99).all())
 
 
+def tie_rows(rows, cols):
+    """float32 rows whose values lie on either side of the steps' middles: the
+    product in fp32 is a middle where the unrounded one is a little off it."""
+    r = np.random.default_rng(cols)
+    top = (1 + r.random((rows, 1))).astype(F32)
+    inv = (F32(127) / top).astype(F32)
+    x = ((r.integers(-127, 127, (rows, cols)) + 0.5) / inv.astype(np.float64)).astype(F32)
+    for _ in range(2):
+        x = np.where(r.random(x.shape) < 0.3, np.nextafter(x, r.choice([F32(-4), F32(4)], x.shape)), x).astype(F32)
+    x = np.clip(x, -top, top)
+    x[:, 0] = top[:, 0]
+    return x, inv
+
+
+@pytest.mark.parametrize("gap", [0, 1])
+@pytest.mark.parametrize("cols", [1000, 4096, 5001])
+def test_products_are_rounded_before_the_whole_number_is_taken(cuda, pz, cols, gap):
+    torch = cuda
+    x, inv = tie_rows(8, cols)
+    want = quantize_ref(x)[0]
+    assert (np.rint(x.astype(np.float64) * inv.astype(np.float64)) != want).sum() > 20   # one rounding moves them
+    xs = torch.zeros(8, cols + gap, device="cuda")[:, :cols]
+    xs.copy_(torch.from_numpy(x).cuda())
+    buf, q = padded(torch, 8, cols)
+    scale = torch.empty(8, device="cuda")
+    pz.quantize_rows_i8(xs, q, scale)
+    assert np.array_equal(q.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [9, 2051, 4103, 9001])
+def test_infinities_and_nan_at_either_end_of_a_row(cuda, pz, cols, dtype):
+    torch = cuda
+    td = torch.float32 if dtype == "f32" else torch.bfloat16
+    xs = torch.ones(5, cols, dtype=td, device="cuda")      # odd: every row at another alignment
+    bad = [(0, 0, np.nan), (1, cols - 1, np.nan), (2, 0, -np.inf), (3, cols - 1, np.inf)]
+    for row, col, v in bad:
+        xs[row, col] = float(v)
+    buf, q = padded(torch, 5, cols)
+    scale = torch.empty(5, device="cuda")
+    pz.quantize_rows_i8(xs, q, scale)
+    assert scale[:4].isnan().all() and (q[:4] == 0).all()
+    assert scale[4].item() == F32(1) / F32(127) and (q[4] == 127).all()
+
+
 SHAPES = [
     # M, N, K
     (1, 1, 1), (1, 130, 33), (2, 127, 128), (3, 129, 16), (15, 300, 100), (16, 128, 256), (17, 1000, 129),
