@@ -170,7 +170,6 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
         id = -1;
         t = -INFINITY;
       } else {
-        if (!REST) t = __fdiv_rn(t, A.T);
         seen++;
         bad |= t != t;
         top = fmaxf(top, t);
@@ -200,7 +199,9 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
     seen += s_seen[i];
     bad |= s_bad[i];
   }
-  // LIST: relative to the largest; REST: as they are
+  // LIST: relative to the largest, the difference before the division by T:
+  // values of the type's lowest or far from zero keep what sets them apart.
+  // REST: as they are.
   const float base = (REST || !(top > -INFINITY)) ? 0.0f : top;
   // A list that names every id leaves none for rho (what 1 - sum holds then
   // is rounding).
@@ -220,7 +221,7 @@ __device__ __forceinline__ List read_list(const DistillArgs &A, int64_t row, con
       const int j = tid + e * kThreads;
       if (j >= A.K) break;
       const int id = L.id[j];
-      const float t = __fsub_rn(L.log_p[j], base);
+      const float t = REST ? L.log_p[j] : __fdiv_rn(__fsub_rn(L.log_p[j], base), A.T);
       const float p = id >= 0 ? expf(t) : 0.0f;
       L.log_p[j] = t;
       L.p[j] = p;

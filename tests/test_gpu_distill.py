@@ -381,3 +381,26 @@ def test_wrapper_refuses(cuda, pz):
     with pytest.raises(pz.PZError):
         pz.distill_loss_grad(big[:4], ids, t, loss, big[1:5])
     assert pz.distill_loss(x[:0], ids[:0], t[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("T", [0.5, 0.01, 1e-3])
+def test_list_values_keep_their_differences_at_any_temperature(cuda, pz, T):
+    """Only the differences of a list's values count: values at the type's
+    lowest (which a division by T < 1 takes to -inf), far from zero beside
+    their differences (which it rounds away), and at either end of the type."""
+    torch = cuda
+    N, V, K = 8, 3000, 12
+    x, ids, t, n, w = make(41, N, V, K, False, odd=False)
+    x *= np.float32(T)                            # student and teacher in units of T
+    t *= np.float32(T)
+    t[0] = LOWEST                                 # a flat list
+    t[1, 3:] = LOWEST                             # padded with the lowest value
+    t[2] -= np.float32(20.0)                      # (rounded here: the oracle sees the same values)
+    t[3] += np.float32(1000.0)
+    t[4] = -LOWEST
+    t[5], t[5, 4] = LOWEST, -LOWEST               # one id takes it all
+    t[6, ::2] = -np.inf
+    for how in ("both", "one"):
+        loss, grad = run(torch, pz, x, ids, t, n, w, T, False, torch.float32, how=how)
+        check(x, ids, t, n, w, T, False, loss, grad, 2.0 ** -24)
+        assert np.isfinite(loss).all() and (loss != 0).all()
