@@ -644,7 +644,9 @@ def configs_to_device(cfg_np, device="cuda"):
 # Rows of logits outside the sampler: constraints, distillation.
 # --------------------------------------------------------------------------
 # (these run at every call of a decode step: torch looked up once, indexes
-# instead of device objects, and torch's raw calls where it hands them out)
+# instead of device objects, and torch's raw calls where it hands them out.
+# All but distill_loss are outside autograd: they have no derivative, and what
+# they write counts as changed in place.)
 class _Torch:
     """torch, its current device and raw current stream, and dtype codes; made
     at the first call, so that importing this module does not import torch."""
@@ -655,6 +657,7 @@ class _Torch:
         self.words = (torch.int32, torch.uint32)
         self.codes = {torch.float32: PZ_DTYPE_F32, torch.bfloat16: PZ_DTYPE_BF16}
         self.device = torch.cuda.device
+        self.written = torch.autograd.graph.increment_version
         self.current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda d: torch.cuda.current_stream(d).cuda_stream)
@@ -674,9 +677,11 @@ def _code(T, t):
     return Sampler._dtype_code(t) if code is None else code  # (which raises)
 
 
-def _call(fn, name, dev, stream, *args):
+def _call(fn, name, dev, stream, written, *args):
     """Calls a context-free entry on device `dev`, on `stream` or that
-    device's current stream."""
+    device's current stream.  `written` are the caller's tensors that it
+    writes: autograd is told, so that a graph that saved one of them refuses
+    its backward pass as it does after torch's own in-place operations."""
     T = _T
     handle = T.raw_stream(dev) if stream is None else _stream_handle(stream)
     if dev == T.current_device():
@@ -686,6 +691,8 @@ def _call(fn, name, dev, stream, *args):
             st = fn(*args, handle)
     if st != PZ_OK:
         raise PZError(st, name)
+    if written:
+        T.written(written)
 
 
 def _rows(t, name, like=None):
@@ -761,8 +768,8 @@ def process_logits(logits, out=None, *, cfg=None, hist=None, hist_off=None, bias
     n_out = _vector(n_allowed, "n_allowed", B, i32, dev)
     if B == 0:
         return out
-    _call(_lib.pz_process_logits, "pz_process_logits", dev, stream, logits.data_ptr(), _code(T, logits),
-          B, V, ld, ctypes.byref(rules), out.data_ptr(), _code(T, out), ld_out, n_out)
+    _call(_lib.pz_process_logits, "pz_process_logits", dev, stream, (out,) if n_allowed is None else (out, n_allowed),
+          logits.data_ptr(), _code(T, logits), B, V, ld, ctypes.byref(rules), out.data_ptr(), _code(T, out), ld_out, n_out)
     return out
 
 
@@ -803,8 +810,8 @@ def distill_forward(logits, ids, values, loss, stats=None, *, weight=None, tempe
     out = _vector(loss, "loss", N, T.f32, dev), _vector(stats, "stats", 4 * N, T.f32, dev)
     if N == 0:
         return loss
-    _call(_lib.pz_distill_forward, "pz_distill_forward", dev, stream, logits.data_ptr(), _code(T, logits),
-          N, V, ld, ctypes.byref(target), *out)
+    _call(_lib.pz_distill_forward, "pz_distill_forward", dev, stream, (loss,) if stats is None else (loss, stats),
+          logits.data_ptr(), _code(T, logits), N, V, ld, ctypes.byref(target), *out)
     return loss
 
 
@@ -819,7 +826,7 @@ def distill_backward(logits, ids, values, stats, grad, grad_loss=None, *, weight
     given = _vector(stats, "stats", 4 * N, T.f32, dev), _vector(grad_loss, "grad_loss", N, T.f32, dev)
     if N == 0:
         return grad
-    _call(_lib.pz_distill_backward, "pz_distill_backward", dev, stream, logits.data_ptr(),
+    _call(_lib.pz_distill_backward, "pz_distill_backward", dev, stream, (grad,), logits.data_ptr(),
           _code(T, logits), N, V, ld, ctypes.byref(target), *given, grad.data_ptr(), ld_grad)
     return grad
 
@@ -835,7 +842,7 @@ def distill_loss_grad(logits, ids, values, loss, grad, *, weight=None, temperatu
     out = _vector(loss, "loss", N, T.f32, dev)
     if N == 0:
         return loss, grad
-    _call(_lib.pz_distill_loss_grad, "pz_distill_loss_grad", dev, stream, logits.data_ptr(),
+    _call(_lib.pz_distill_loss_grad, "pz_distill_loss_grad", dev, stream, (loss, grad), logits.data_ptr(),
           _code(T, logits), N, V, ld, ctypes.byref(target), out, grad.data_ptr(), ld_grad)
     return loss, grad
 
@@ -858,7 +865,7 @@ def _distill_function():
                 loss = torch.empty(N, dtype=T.f32, device=logits.device)
                 stats = torch.empty(N, 4, dtype=T.f32, device=logits.device)
                 if N:
-                    _call(_lib.pz_distill_forward, "pz_distill_forward", dev, None, logits.data_ptr(),
+                    _call(_lib.pz_distill_forward, "pz_distill_forward", dev, None, None, logits.data_ptr(),
                           _code(T, logits), N, V, ld, ctypes.byref(target), loss.data_ptr(),
                           stats.data_ptr())
                 ctx.save_for_backward(logits, ids, values, weight, n_list, stats)
@@ -873,7 +880,7 @@ def _distill_function():
                 grad = torch.empty(N, V, dtype=logits.dtype, device=logits.device)
                 if N:
                     grad_loss = grad_loss.contiguous()
-                    _call(_lib.pz_distill_backward, "pz_distill_backward", dev, None, logits.data_ptr(),
+                    _call(_lib.pz_distill_backward, "pz_distill_backward", dev, None, None, logits.data_ptr(),
                           _code(T, logits), N, V, ld, ctypes.byref(target), stats.data_ptr(),
                           grad_loss.data_ptr(), grad.data_ptr(), V)
                 return grad, None, None, None, None, None, None
@@ -913,7 +920,7 @@ def quantize_rows_i8(x, q, scale, stream=None):
     out = _vector(scale, "scale", rows, T.f32, dev)
     if rows == 0:
         return q, scale
-    _call(_lib.pz_quantize_rows_i8, "pz_quantize_rows_i8", dev, stream, x.data_ptr(), _code(T, x), rows,
+    _call(_lib.pz_quantize_rows_i8, "pz_quantize_rows_i8", dev, stream, (q, scale), x.data_ptr(), _code(T, x), rows,
           cols, ld, q.data_ptr(), ld_q, out)
     return q, scale
 
@@ -929,7 +936,7 @@ def matmul_i8(a, a_scale, w, w_scale, out, stream=None):
     scales = (_vector(a_scale, "a_scale", M, T.f32, dev), _vector(w_scale, "w_scale", N, T.f32, dev))
     if M == 0:
         return out
-    _call(_lib.pz_matmul_i8, "pz_matmul_i8", dev, stream, a.data_ptr(), ld_a, scales[0], M, w.data_ptr(), ld_w,
+    _call(_lib.pz_matmul_i8, "pz_matmul_i8", dev, stream, (out,), a.data_ptr(), ld_a, scales[0], M, w.data_ptr(), ld_w,
           scales[1], N, K, out.data_ptr(), _code(T, out), ld)
     return out
 
@@ -950,7 +957,7 @@ def lm_head_i8(hidden, w_q, w_scale, logits, hidden_q, hidden_scale, stream=None
               _vector(hidden_scale, "hidden_scale", B, T.f32, dev))
     if B == 0:
         return logits
-    _call(_lib.pz_lm_head_logits_i8, "pz_lm_head_logits_i8", dev, stream, hidden.data_ptr(),
-          _code(T, hidden), B, dim, ld_hidden, w_q.data_ptr(), ld_w, scales[0], V, logits.data_ptr(),
-          _code(T, logits), ld, hidden_q.data_ptr(), ld_q, scales[1])
+    _call(_lib.pz_lm_head_logits_i8, "pz_lm_head_logits_i8", dev, stream, (logits, hidden_q, hidden_scale),
+          hidden.data_ptr(), _code(T, hidden), B, dim, ld_hidden, w_q.data_ptr(), ld_w, scales[0], V,
+          logits.data_ptr(), _code(T, logits), ld, hidden_q.data_ptr(), ld_q, scales[1])
     return logits
