@@ -17,6 +17,7 @@
 
 #include <atomic>
 
+#include "pz_epilogue.cuh"
 #include "pz_rowvec.cuh"
 #include "pz_status.cuh"
 #include "pz_tcgen05.cuh"
@@ -169,11 +170,13 @@ struct MatmulArgs {
 // 16.3 with four).
 //
 // Rows and K past the matrices' ends arrive as zeros.  Every wait is bounded:
-// one that runs out (4 s; nothing in this kernel can cause it) ends the CTA
-// after its loads have landed and its products are done, with NaN in the
-// outputs it did not reach.
+// one that runs out (4 s: no work of this kernel takes as long, a GPU that was
+// held in between does) ends the CTA after its loads have landed and its products
+// are done, with NaN in the outputs it did not reach: every warp of the
+// epilogue fills its own tokens.
 // ---------------------------------------------------------------------------
-constexpr int kTcWarps = 8;           // of the epilogue
+using OwnTokens = EpilogueTokens<8>;  // of each of the epilogue's warps
+constexpr int kTcWarps = OwnTokens::WARPS;
 constexpr int kTcThreads = 64 + 32 * kTcWarps;
 constexpr int kTcChannels = 128;
 constexpr int kTcTokens = 256;
@@ -364,8 +367,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncwarp();
   } else {
     pdl_wait();
-    const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
-    const int first = (warp - 2) / 4 * 32;  // its first token; two warps share a quarter, 32 tokens in turn
+    const int quarter = OwnTokens::quarter(warp);
+    const int first = OwnTokens::first(warp - 2);
     const int row = quarter * 32 + lane;
     int t = 0;
     bool ok = true;
@@ -382,28 +385,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (ok) ok = mbar_wait(sum + 8 * acc, (t >> 1) & 1, &s_stop);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) {
-        for (int j = 0; j < tokens; j++)
-          if (n < A.N && first == 0) RowElem<T>::put(out + static_cast<int64_t>(j) * A.ld_out, __int_as_float(0x7FC00000));
+        for (int c = first; c < tokens; c += OwnTokens::STEP)
+          for (int j = 0; j < OwnTokens::count(c, tokens); j++)
+            if (n < A.N) RowElem<T>::put(out + static_cast<int64_t>(c + j) * A.ld_out, __int_as_float(0x7FC00000));
         continue;
       }
       tc_fence_after();
       const uint32_t at = tmem + static_cast<uint32_t>(acc * (A.cols / 2)) + (static_cast<uint32_t>(quarter * 32) << 16);
       // 32 tokens at a time; each lane fetches one token's scale, ahead of
       // the stores that the compiler may not move a load across
-      constexpr int STEP = 8 * kTcWarps;
-      for (int c = first; c < tokens; c += STEP) {
+      for (int c = first; c < tokens; c += OwnTokens::STEP) {
         int v[32];
         __syncwarp();
         tmem_load32(at + c, v);
         const float here = sa;
-        if (c + STEP + lane < tokens) sa = __ldcg(A.a_scale + m0 + c + STEP + lane);
+        if (c + OwnTokens::STEP + lane < tokens) sa = __ldcg(A.a_scale + m0 + c + OwnTokens::STEP + lane);
         tmem_load_wait();
         float x[32];
 #pragma unroll
         for (int j = 0; j < 32; j++)
           x[j] = __fmul_rn(__int2float_rn(v[j]), __fmul_rn(__shfl_sync(0xFFFFFFFFu, here, j), sw));
         T *o = out + static_cast<int64_t>(c) * A.ld_out;
-        if (c + 32 <= tokens) {
+        if (OwnTokens::count(c, tokens) == OwnTokens::RUN) {
           if (n < A.N) {
 #pragma unroll
             for (int j = 0; j < 32; j++) RowElem<T>::put(o + j * A.ld_out, x[j]);
