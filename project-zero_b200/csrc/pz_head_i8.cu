@@ -171,8 +171,8 @@ struct MatmulArgs {
 //
 // Rows and K past the matrices' ends arrive as zeros.  Every wait is bounded:
 // one that runs out (4 s: no work of this kernel takes as long, a GPU that was
-// held in between does) ends the CTA after its loads have landed and its products
-// are done, with NaN in the outputs it did not reach: every warp of the
+// held in between does) ends the CTA once its products are done and its loads
+// have landed, with NaN in the outputs it did not reach: every warp of the
 // epilogue fills its own tokens.
 // ---------------------------------------------------------------------------
 using OwnTokens = EpilogueTokens<8>;  // of each of the epilogue's warps
@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (PAIR) pair_sync();  // the other CTA's barriers are set up too
   tc_fence_after();
   const uint32_t tmem = s_tmem;
+  int64_t loads = 0;  // stages that this thread has loaded
 
   if (warp == 0) {
     if (lane == 0) {
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       pdl_wait();
-      int64_t n = 0;
+      int64_t n = 0;  // (loads)
       uint32_t slot = ring, bar = full, gone = empty, ph = 1;
       const uint32_t ring_end = ring + A.stages * stage_bytes;
       bool ok = true;
@@ -303,15 +304,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // no commit may be on its way to this CTA's barriers when its memory goes
       for (int64_t i = n < A.stages ? 0 : n - A.stages; ok && PAIR && i < n; i++)
         ok = mbar_wait(empty + 8 * static_cast<uint32_t>(i % A.stages), static_cast<uint32_t>((i / A.stages) & 1), &s_stop);
-      // after a stop: no load may be in flight when the CTA's memory goes (the
-      // leading CTA waits for both CTAs' loads)
-      if (s_stop && rank == 0) {
-        const int64_t last = n < A.stages ? n : A.stages;
-        for (int64_t i = n - last; i < n; i++) {
-          volatile int ignore = 0;
-          mbar_wait(full + 8 * static_cast<uint32_t>(i % A.stages), static_cast<uint32_t>((i / A.stages) & 1), &ignore);
-        }
-      }
+      loads = n;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -358,11 +351,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (ok) tc_commit<PAIR>(sum + 8 * acc);
       }
-      if (s_stop) {
-        volatile int ignore = 0;
-        tc_commit<PAIR>(smem_addr(&s_drain));
-        mbar_wait(smem_addr(&s_drain), 0, &ignore);
-      }
+      // no product may be under way when the CTA's memory goes, whether or not
+      // the epilogue waited for it (where it did, this costs nothing)
+      tc_commit<PAIR>(smem_addr(&s_drain));
+      volatile int ignore = 0;
+      mbar_wait(smem_addr(&s_drain), 0, &ignore);
     }
     __syncwarp();
   } else {
@@ -425,6 +418,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  // After a stop: no load may be in flight when the CTA's memory goes (the
+  // leading CTA waits for both CTAs' loads; without a stop its products have).
+  // Only here is it known whether any role stopped.
+  if (s_stop && rank == 0 && tid == 0) {
+    for (int64_t i = loads < A.stages ? 0 : loads - A.stages; i < loads; i++) {
+      volatile int ignore = 0;
+      mbar_wait(full + 8 * static_cast<uint32_t>(i % A.stages), static_cast<uint32_t>((i / A.stages) & 1), &ignore);
+    }
+  }
+  if (PAIR && rank == 1 && tid == 32) {  // nor the leading CTA's signal, which arrives here too
+    volatile int ignore = 0;
+    mbar_wait(smem_addr(&s_drain), 0, &ignore);
+  }
   if (PAIR) pair_sync();  // neither CTA's memory or barriers are used by the other any more
   if (warp == 2) {
     tc_fence_after();
