@@ -466,7 +466,8 @@ pz_status pz_distill_loss_grad(const void *logits, pz_dtype dtype, int N, int V,
  * (hidden_q [B x dim], hidden_scale [B]; overwritten, so two calls in flight
  * need two of them).
  * 8-bit matrices start on a 16-byte boundary and so does each of their rows
- * (ld_* multiples of 16); what lies between K and ld is not read.
+ * (ld_* multiples of 16); what lies between K and ld is not read.  Up to
+ * 2^31 - 16 columns are quantised, up to 2^31 - 256 rows multiplied.
  * The product's kernel bounds its waits at 4 s.  One that runs out (no work of
  * its own takes as long; a GPU that is held meanwhile can) leaves NaN in the
  * outputs that were not reached, the call having returned PZ_OK. */

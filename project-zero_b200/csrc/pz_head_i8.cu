@@ -545,6 +545,10 @@ cudaError_t launch_matmul(const MatmulArgs &A, pz_dtype out_dtype, bool after_qu
                                    : launch_matmul_to<bf16_t>(A, after_quantize, st);
 }
 
+// Largest sizes that still fit 32-bit indexes when they are rounded up to a
+// vector (columns of a row) or a tile (tokens, channels).
+constexpr int kMaxCols = 0x7FFFFFFF - 15, kMaxTiled = 0x7FFFFFFF - 255;
+
 pz_status check_quantize(const void *x, pz_dtype dtype, int rows, int cols, int64_t ld, const int8_t *q, int64_t ld_q,
                          const float *scale) {
   if (!x || !q || !scale || rows < 0 || cols <= 0 || ld < cols || ld_q < cols)
@@ -555,6 +559,7 @@ pz_status check_quantize(const void *x, pz_dtype dtype, int rows, int cols, int6
     return report(PZ_ERR_INVALID_ARGS, "pz_quantize_rows_i8: q and its rows start on 16 bytes, x on its elements");
   if (rows > 0 && overlap(x, rows_bytes(rows, cols, ld, elem_bytes(dtype)), q, rows_bytes(rows, cols, ld_q, 1)))
     return report(PZ_ERR_INVALID_ARGS, "pz_quantize_rows_i8: q lies over x");
+  if (cols > kMaxCols) return report(PZ_ERR_UNSUPPORTED, "pz_quantize_rows_i8: more than 2^31 - 16 columns");
   return PZ_OK;
 }
 
@@ -574,6 +579,8 @@ pz_status check_matmul(const MatmulArgs &A, pz_dtype out_dtype) {
     return report(PZ_ERR_INVALID_ARGS, "pz_matmul_i8: out lies over a or w");
   if (A.K >= PZ_MATMUL_I8_MAX_K)
     return report(PZ_ERR_UNSUPPORTED, "pz_matmul_i8: K of 2^17 or more may overflow the 32-bit sums");
+  if (A.M > kMaxTiled || A.N > kMaxTiled)
+    return report(PZ_ERR_UNSUPPORTED, "pz_matmul_i8: more than 2^31 - 256 rows");
   return PZ_OK;
 }
 

@@ -107,3 +107,19 @@ def test_head_limits_and_empty():
     assert L.pz_matmul_i8(P, 64, None, 2, P * 2, 64, P, 10, 64, P * 3, 0, 10, None) == BAD
     assert L.pz_quantize_rows_i8(P, 0, 0, 64, 64, P, 64, P, None) == OK
     assert L.pz_quantize_rows_i8(P, 0, 2, 64, 64, P, 60, P, None) == BAD
+
+
+def test_sizes_that_32_bit_indexes_do_not_hold():
+    """Rounded up to a vector or a tile they would wrap: an unwritten row with
+    scale 0, a grid of a negative size."""
+    top = (1 << 31) - 1
+    far = 1 << 40
+    for cols in (top, top - 14):
+        assert L.pz_quantize_rows_i8(P, 0, 1, cols, 1 << 31, far, 1 << 31, P, None) == UNSUPPORTED
+        assert b"2^31" in L.pz_last_error_detail()
+    for n in (top, top - 254):
+        assert L.pz_matmul_i8(P, 16, P, 1, far, 16, P, n, 16, far * 2, 0, 1 << 31, None) == UNSUPPORTED
+        assert L.pz_matmul_i8(far, 16, P, n, P, 16, P, 1, 16, far * 2, 0, 1 << 31, None) == UNSUPPORTED
+        assert b"2^31" in L.pz_last_error_detail()
+    assert L.pz_quantize_rows_i8(P, 0, 0, top - 15, 1 << 31, far, 1 << 31, P, None) == OK
+    assert L.pz_matmul_i8(P, 16, P, 0, far, 16, P, top - 255, 16, far * 2, 0, 1 << 31, None) == OK
