@@ -359,7 +359,10 @@ pz_status pz_decode_step_destroy(pz_decode_step *step);
  * may be captured into a graph, and calls on different streams may overlap
  * as long as their outputs are apart.  Rows are given like pz_sample_batch's
  * (row r at + r*ld elements, any ld >= V, any address that is a multiple of
- * the element's size).  An empty batch (0 rows) is PZ_OK. */
+ * the element's size).  An output row is stored 16 bytes at a time where it
+ * lies at the same offset from a 16-byte boundary as the input's row, an
+ * element at a time elsewhere (bf16: up to four times as long): give outputs
+ * of padded rows the same ld.  An empty batch (0 rows) is PZ_OK. */
 
 /* What is applied to each row of logits, in this order.  Device pointers;
  * each group may be NULL (off).
@@ -397,7 +400,9 @@ typedef struct pz_logits_rules {
  * number of ids the row's mask allows (V without a mask): 0 tells a row that
  * is all -inf, which the samplers treat as they treat any such row.
  * pz_sample_batch on an f32 `out` without a history draws what it would draw
- * from the logits with the history. */
+ * from the logits with the history.  A sampling call (pz_decode_step's too)
+ * that is given a history applies its penalties after these biases and masks:
+ * let one of the two have it. */
 pz_status pz_process_logits(const void *logits, pz_dtype dtype, int B, int V, int64_t ld,
                             const pz_logits_rules *rules, void *out, pz_dtype out_dtype,
                             int64_t ld_out, int32_t *n_allowed, void *stream);
@@ -418,8 +423,10 @@ pz_status pz_process_logits(const void *logits, pz_dtype dtype, int B, int V, in
  * has no entries left or, in LIST mode, only values of -inf, has loss and
  * gradient 0, whatever its logits.  A row of logits that are all -inf has
  * loss +inf and gradient 0; a listed id the student gives -inf has loss +inf
- * where its p > 0.  NaN in the logits or in the values of a row makes its
- * loss and gradient NaN. */
+ * where its p > 0.  So has a row whose ids off the list are all -inf while
+ * rho > 0, and what rounding leaves of 1 - sum p counts: where the list holds
+ * all ids that a mask allows, use PZ_DISTILL_LIST.  NaN in the logits or in
+ * the values of a row makes its loss and gradient NaN. */
 #define PZ_DISTILL_LIST 0
 #define PZ_DISTILL_REST 1
 #define PZ_DISTILL_MAX_VOCAB 1048576

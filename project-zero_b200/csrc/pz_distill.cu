@@ -18,8 +18,10 @@
 //
 // Everything runs in units of 2: e_v = 2^((s_v - m) c), c = log2(e) / T, m a
 // maximum (the difference first, so rows of the type's lowest value keep
-// their shape).  Sums of e are fp32, at most a few hundred terms per thread,
-// joined in a fixed order: the same call gives the same bits.  REST keeps
+// their shape).  Sums of e are fp32, joined in a fixed order: the same call
+// gives the same bits.  A thread adds the even and the odd columns apart, 501
+// terms each for a row of 128256 in one CTA, 768 for the longest span that a
+// CTA's bits allow (196608 columns), and scales the sums once a batch.  REST keeps
 // the ids off the list under a maximum of their own, so that log r and
 // rho / r hold when the student leaves them next to nothing.  The sum over
 // the list, whose terms nearly cancel against log S, is in fp64.
@@ -29,18 +31,24 @@
 // not hide altogether.
 //   loss      a row per CTA while the rows fill the GPU, parts of one in a
 //             cluster otherwise; the next batch of vectors in flight while one
-//             is summed.  1024 rows of 128256 f32: 74 us, 7.1 TB/s.
+//             is summed.  1024 rows of 128256 f32, nine tenths of them with
+//             a weight (the others are not read, here and below): 74 us, 6.4
+//             TB/s.
 //   gradient  from saved statistics: parts of 64 KB, independent CTAs.  2048
-//             rows of 151936 bf16: 190 us, 6.5 TB/s (after a loss of 99 us).
+//             rows of 151936 bf16: 190 us, 6.2 TB/s (after a loss of 99 us).
 //   both      one read and one write: a row stays on chip between its two
 //             passes.  A cluster of up to 8 CTAs takes it, each fetching 32 KB
 //             of it into shared memory (cp.async; a thread reads back what it
 //             fetched itself), and they exchange maximum and sums through
 //             distributed shared memory.  4096 rows of 128256 bf16: 412 us,
-//             5.1 TB/s.  Four warps a CTA: with eight, each repeating the
+//             4.8 TB/s.  Four warps a CTA: with eight, each repeating the
 //             row's scalars for half as many columns, it was 566 us, with two
 //             495; parts of 64 KB (three CTAs on an SM, not five) 505.
 // The list is read by all parts of its row: at most 1024 ids, two barriers.
+// Gradient rows that lie at another offset from a 16-byte boundary than the
+// logits' are stored an element at a time: 2048 rows of 50257 bf16, logits
+// 50304 apart, gradient alone 269 us where its rows are contiguous, 74 where
+// they are 50304 apart too.
 #include <atomic>
 
 #include "pz_device.cuh"

@@ -117,8 +117,15 @@ __global__ void __launch_bounds__(NT) quantize_kernel(const QuantArgs A) {
 // 128 threads while their registers hold the row (8 KB), 256 beyond.  Both
 // sides, 128 and 256 threads, us: 128256 x 4096 bf16 235 and 357, 32000 x 1000
 // bf16 36 and 66, 1024 x 4096 bf16 3.3 and 4.3; 128256 x 8192 bf16 666 and 489,
-// 512 x 4096 f32 4.1 and 3.0, 1 x 4096 f32 3.3 and 2.0.  Threads in a number
-// set at run time to fit each row were slower than the better of the two.
+// 128256 x 6144 bf16 473 and 421, 128256 x 3000 f32 389 and 328, 512 x 4096 f32
+// 4.1 and 3.0, 1 x 4096 f32 3.3 and 2.0.  From 8 to about 11 KB the narrow side
+// still wins where rows are many (128256 x 2560 f32 272 and 297, 128256 x 5120
+// bf16 351 and 391) and loses on a batch of tokens whose rows come from memory
+// (1024 x 2560 f32 10.1 and 8.2): tokens are quantised at every call, a
+// classifier once.  Threads in a number set at run time to fit each row were
+// slower than the better of the two.  Rows of 2 KB are bound by the start and
+// the end of a CTA each, 2.4 times their bytes' time.  Rows at odd addresses
+// are stored a byte at a time (32000 x 1001 bf16 62 us, 32000 x 1000 37).
 template <typename T>
 void launch_quantize_as(const QuantArgs &A, cudaStream_t st) {
   constexpr int narrow_cols = 128 * kQuantRes * RowElem<T>::N;
@@ -153,7 +160,7 @@ struct MatmulArgs {
 //
 // Few tokens: bound by HBM, every weight read once: a persistent CTA per SM
 // keeps about 200 KB of weights and tokens in flight (1 token, dim 2560,
-// 128256 channels: 53 us, 6.3 TB/s; 64 tokens, dim 4096, 151936 channels: 108
+// 128256 channels: 53 us, 6.2 TB/s; 64 tokens, dim 4096, 151936 channels: 108
 // us, 6.1 TB/s).  Many tokens: bound by what the SMs fetch from L2 (54 bytes a
 // clock each, measured; a tile of 128 x 256 wants 384 bytes per 32768
 // products, half a tile in a pair of CTAs 256), and beside it by the tensor

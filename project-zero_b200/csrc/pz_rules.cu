@@ -14,11 +14,17 @@
 //   mask      v's bit is 0: x = -inf, whatever x was (NaN and inf included)
 //
 // Bound: HBM.  Out of place every logit is read and written once (1024 rows of
-// 128256 f32: 165 us without rules, 5.3 TB/s of a copy's 6.5; 167 with masks;
-// 199 with 1024 history ids a row, each of which is another 32-byte sector to
-// fetch and to write).  In place only the vectors that something changes are
-// touched: 4096 rows of 151936 bf16 under masks, half of them random, 343 us;
-// a sector that a mask takes part of is read and written whole, 1.65 GB there.
+// 128256 f32: 165 us without rules, 6.4 TB/s of a copy's 6.5; 167 with masks;
+// 199, 5.3 TB/s, with 1024 history ids a row, each of which is another 32-byte
+// sector to fetch and to write; bf16 into f32 153 with masks and 166 with
+// lists too).  In place only the vectors that something changes are touched:
+// 4096 rows of 151936 bf16 under masks, half of them random, 343 us; a sector
+// that a mask takes part of is read and written whole, 1.65 GB there.  Under
+// masks and lists together it is no gain: the 1024 f32 rows 241 us (74 with
+// the lists alone, 137 with the masks).  Rows of out that lie at another offset
+// from a 16-byte boundary than the logits' are stored an element at a time
+// (1024 rows of 128255, odd addresses into rows 128256 apart: f32 184 us
+// against 172, bf16 352 against 90).
 //
 // A CTA takes a part of a row.  Four warps pass along its columns and know
 // the mask alone.  Two more work out the listed ids meanwhile: those that lie

@@ -891,8 +891,11 @@ def _distill_function():
 
 def distill_loss(logits, ids, values, *, weight=None, temperature=1.0, mode=DISTILL_LIST, n_list=None):
     """The row losses [N] of distill_forward, differentiable in the logits
-    (not in the teacher's values or the weights).  Runs on the current
-    stream; the gradient is one more pass over the logits."""
+    (not in the teacher's values or the weights, which get no gradient).  Runs
+    on the current stream; the gradient is one more pass over the logits, into
+    contiguous rows (logits that are a view of padded rows take longer).  A
+    backward pass may be captured into a graph while no eager graph of the
+    same leaves lives, as with torch's own operations."""
     return _distill_function().apply(logits, ids, values, weight, temperature, mode, n_list)
 
 

@@ -404,3 +404,19 @@ def test_list_values_keep_their_differences_at_any_temperature(cuda, pz, T):
         loss, grad = run(torch, pz, x, ids, t, n, w, T, False, torch.float32, how=how)
         check(x, ids, t, n, w, T, False, loss, grad, 2.0 ** -24)
         assert np.isfinite(loss).all() and (loss != 0).all()
+
+
+def test_a_student_masked_off_the_list(cuda, pz):
+    """Every id off the list is -inf: REST holds what the list leaves against
+    nothing (loss +inf, a gradient on the list alone), LIST is finite."""
+    torch = cuda
+    N, V, K = 4, 4001, 9
+    x, ids, t, n, w = make(51, N, V, K, True, odd=False)
+    on = np.zeros((N, V), dtype=bool)
+    np.put_along_axis(on, ids, True, 1)
+    x[~on] = -np.inf
+    for rest in (True, False):
+        for how in ("both", "one"):
+            loss, grad = run(torch, pz, x, ids, t, n, w, 1.0, rest, torch.float32, how=how)
+            check(x, ids, t, n, w, 1.0, rest, loss, grad, 2.0 ** -24)
+            assert (loss == np.inf).all() == rest and np.isfinite(grad).all() and not grad[~on].any()
