@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(NT) quantize_kernel(const QuantArgs A) {
 // (1024 x 2560 f32 10.1 and 8.2): tokens are quantised at every call, a
 // classifier once.  Threads in a number set at run time to fit each row were
 // slower than the better of the two.  Rows of 2 KB are bound by the start and
-// the end of a CTA each, 2.4 times their bytes' time.  Rows at odd addresses
+// the end of a CTA each, 2.5 times their bytes' time.  Rows at odd addresses
 // are stored a byte at a time (32000 x 1001 bf16 62 us, 32000 x 1000 37).
 template <typename T>
 void launch_quantize_as(const QuantArgs &A, cudaStream_t st) {
